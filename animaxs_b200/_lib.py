@@ -87,11 +87,32 @@ class ProjDesc(ctypes.Structure):
     ]
 
 
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("capacity", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("format", ctypes.c_int32),
+        ("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class Kv8WriteDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int32), ("start", ctypes.c_int32),
+        ("starts", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+        ("k_tok_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("k_batch_stride", ctypes.c_int64),
+        ("v_tok_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("v_batch_stride", ctypes.c_int64),
+    ]
+
+
+KV8_INT8, KV8_E4M3 = 0, 1
+KV8_BLOCK_TOKENS = 64
+
 PROJ_STORE, PROJ_QKV_NORM, PROJ_GATE_ADD = 0, 1, 2
 WEIGHT_FP16, WEIGHT_W8, WEIGHT_W4 = 0, 1, 2
 
 # name -> (restype, argtypes); every symbol the header declares.
-ABI_VERSION = 3  # ANIMAXS_ATTN_ABI_VERSION in include/animaxs_attn.h
+ABI_VERSION = 4  # ANIMAXS_ATTN_ABI_VERSION in include/animaxs_attn.h
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -138,6 +159,12 @@ SIGNATURES = {
                                           ctypes.POINTER(_I64), ctypes.POINTER(_I)]),
     "animaxs_cross_kv_cache_mark_ready": (_I, [_P, _I, _I]),
     "animaxs_cross_kv_cache_reset": (_I, [_P]),
+    "animaxs_kv8_cache_bytes": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
+    "animaxs_kv8_write": (_I, [_P, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8WriteDesc), _P, _P, _P]),
+    "animaxs_kv8_write_validate": (_I, [_P, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8WriteDesc), _P, _P]),
+    "animaxs_kv8_read": (_I, [_P, ctypes.POINTER(Kv8Cache), _I, _I, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "animaxs_kv8_attn_forward": (_I, [_P, ctypes.POINTER(Kv8Cache), _DESC, _P, _P, _P]),
+    "animaxs_kv8_attn_validate": (_I, [_P, ctypes.POINTER(Kv8Cache), _DESC, _P, _P]),
     "animaxs_weight_streamer_create": (_I, [_P, _I64, _I, ctypes.POINTER(_P)]),
     "animaxs_weight_streamer_destroy": (_I, [_P]),
     "animaxs_weight_streamer_register_host": (_I, [_P, _P, _I64]),

@@ -27,6 +27,10 @@ struct animaxs_attn_ctx {
   size_t scratch_bytes = 0;
   void* staging = nullptr;        // head-sharded path: per-rank slice + gather buffer
   size_t staging_bytes = 0;
+  float* kv8_part = nullptr;           // partial results of split 8-bit-cache attention
+  size_t kv8_part_bytes = 0;
+  unsigned int* kv8_count = nullptr;   // arrivals per split item, zero between calls
+  size_t kv8_count_n = 0;
   unsigned int* d_status = nullptr;  // device status word written by kernels
   int64_t query_tiles = 0;
   bool timing = false;                        // bracket each attention kernel with events
@@ -51,6 +55,10 @@ int ax_validate(animaxs_attn_ctx* ctx, const animaxs_attn_desc* d, const void* q
                 const void* v, const void* o);
 int ax_make_tmap(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,
                  int64_t heads, int64_t batch, int64_t st, int64_t sh, int64_t sb, int box_rows = 128);
+// [heads][rows][dim] bytes, packed (dim 64 or 128); box = dim bytes x box_rows rows,
+// swizzled by the row length (64 or 128 bytes).
+int ax_make_tmap_codes(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,
+                       int64_t heads, int box_rows);
 // Peers of a fused head-sharded call: the epilogue stores every output tile
 // also at o + delta[i] and the CTAs count their items on arrive[i].
 struct AxPeers {

@@ -107,6 +107,8 @@ extern "C" int animaxs_attn_destroy(animaxs_attn_ctx* ctx) {
   cudaDeviceSynchronize();
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->staging) cudaFree(ctx->staging);
+  if (ctx->kv8_part) cudaFree(ctx->kv8_part);
+  if (ctx->kv8_count) cudaFree(ctx->kv8_count);
   if (ctx->d_status) cudaFree(ctx->d_status);
   for (cudaEvent_t e : ctx->events) cudaEventDestroy(e);
   cudaSetDevice(prev);
@@ -293,6 +295,24 @@ int ax_make_tmap(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int6
   if (r != CUDA_SUCCESS)
     return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)",
                         static_cast<int>(r));
+  return ANIMAXS_OK;
+}
+
+int ax_make_tmap_codes(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,
+                       int64_t heads, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr)
+    return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(dim * rows)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(dim), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
   return ANIMAXS_OK;
 }
 
@@ -502,6 +522,9 @@ extern "C" int animaxs_attn_synchronize(animaxs_attn_ctx* ctx, void* stream) {
   unsigned int status = 0;
   if (e == cudaSuccess) e = cudaMemcpy(&status, ctx->d_status, sizeof(status), cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && status != 0) e = cudaMemset(ctx->d_status, 0, sizeof(status));
+  // A kernel that gave up may have left arrivals of a split item uncounted.
+  if (e == cudaSuccess && status != 0 && ctx->kv8_count != nullptr)
+    e = cudaMemset(ctx->kv8_count, 0, ctx->kv8_count_n * sizeof(unsigned int));
   cudaSetDevice(prev);
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "synchronize");
   if (status & ax::kStatusTimeoutBit)

@@ -146,6 +146,56 @@ int proj_kernel_attributes(int* regs, int* max_threads, int* smem_static, int* s
 // [rows][64][2][2] table blocks -> [64][rows] (cos, sin) pairs in `out` (rows*512 bytes).
 cudaError_t launch_rope_pairs(const float* table, void* out, int rows, cudaStream_t stream);
 
+// ---- 8-bit K/V cache (kv8_cache.cu, kv8_rows_sm100.cu) ----
+constexpr int kKv8Block = 64;  // tokens that share a scale
+
+struct Kv8WriteParams {
+  int format, head_dim, batch, kv_heads, capacity, tokens, start;
+  const int* starts;  // per sequence, or nullptr
+  const int* counts;
+  const __half* src[2];  // k, v
+  long long tok[2], head[2], bat[2];
+  uint8_t* codes[2];
+  float* scale[2];
+};
+cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream);
+
+struct Kv8ReadParams {
+  int format, head_dim, batch, kv_heads, capacity, start, tokens;
+  const int* lens;  // per sequence, or nullptr
+  const uint8_t* codes[2];
+  const float* scale[2];
+  __half* out[2];
+  long long tok, head, bat;
+};
+cudaError_t launch_kv8_read(const Kv8ReadParams& p, cudaStream_t stream);
+
+struct Kv8AttnParams {
+  int format, head_dim, batch, kv_heads, group;  // group = query heads per kv head
+  int q_len, kv_len, capacity, n_blocks;         // n_blocks = scales per head
+  int kv_valid;                                  // length of every sequence without lens
+  const int* lens;                               // DEVICE per-sequence lengths, or nullptr
+  int causal;
+  float scale_log2;
+  const __half* q;
+  long long q_tok, q_head, q_batch;
+  __half* o;
+  long long o_tok, o_head, o_batch;
+  const float* k_scale;
+  const float* v_scale;
+  int rows;             // group * q_len: query rows of a kv head
+  int row_tiles;        // 16-row tiles of them
+  float* part;          // workspace: two slots per CTA (kv8_rows_part_floats)
+  unsigned int* count;  // arrivals per (sequence, kv head, row tile), zero between launches
+  unsigned int* status;
+};
+// Attention over the cache in tiles of 16 query rows (kv8_rows_sm100.cu); tk/tv
+// are ax_make_tmap_codes maps with 64-row boxes.
+int kv8_rows_grid(const Kv8AttnParams& p, int sms);
+size_t kv8_rows_part_floats(int head_dim, int grid);
+cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid,
+                            int dev, cudaStream_t stream);
+
 // W8 (bits 8) / W4 (bits 4) codes + fp16 scale/zero per row and 64 columns ->
 // fp16 [rows][out_stride] (dequant_sm100.cu).
 cudaError_t launch_dequant(int bits, const void* packed, const void* scale, const void* zero, void* out,

@@ -1,0 +1,205 @@
+// kv8_cache.cu -- writing the 8-bit K/V cache and reading it back
+// (animaxs_kv8_write, animaxs_kv8_read in include/animaxs_attn.h).
+//
+// Both are streams: 2 bytes in and 1 out per value (write), 1 in and 2 out
+// (read), so HBM bounds them when there is enough to move and the latency of
+// one dependent chain (positions -> rows -> maximum -> codes) when there is not.
+#include "kernels.h"
+#include "kv8_common.cuh"
+
+namespace ax {
+namespace {
+
+constexpr int kWriteThreads = 128;
+
+// The magnitudes of a pair, 0 in place of what is not finite.
+__device__ __forceinline__ __half2 finite_abs(uint32_t w) {
+  const __half2 a = __habs2(*reinterpret_cast<const __half2*>(&w));
+  const __half2 inf = __halves2half2(__ushort_as_half(0x7C00), __ushort_as_half(0x7C00));
+  const uint32_t m = __hlt2_mask(a, inf) & *reinterpret_cast<const uint32_t*>(&a);  // NaN compares false
+  return *reinterpret_cast<const __half2*>(&m);
+}
+// A pair with 0 in place of NaN.
+__device__ __forceinline__ uint32_t nan_to_zero(uint32_t w) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return __heq2_mask(h, h) & w;
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t quantise4(uint32_t a, uint32_t b, float inv) {
+  a = nan_to_zero(a);
+  b = nan_to_zero(b);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  return kv8_pack4<FMT>(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
+}
+
+// One CTA per (64-token block, head, sequence, K or V): it alone reads and
+// writes that block's codes and scale.  A thread keeps its 8-value shares of
+// all the block's rows in registers between the maximum and the rounding, so
+// the source is read once.
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8WriteParams p, int window) {
+  constexpr int kLanes = HD / 8;                       // threads per row
+  constexpr int kRowsPerPass = kWriteThreads / kLanes;
+  constexpr int kPasses = kKv8Block / kRowsPerPass;
+  __shared__ float warp_max[kWriteThreads / 32];
+  int w = blockIdx.x;
+  const int kv = w & 1;
+  w >>= 1;
+  const int h = w % p.kv_heads;
+  w /= p.kv_heads;
+  const int b = w / window;
+  const int wi = w % window;
+  const long long start = p.starts != nullptr ? p.starts[b] : p.start;
+  const int n = p.counts != nullptr ? min(max(p.counts[b], 0), p.tokens) : p.tokens;
+  const long long first = start > 0 ? start : 0;                               // first written position
+  const long long end = start + n < p.capacity ? start + n : p.capacity;       // one past the last
+  const long long blk0 = (first / kKv8Block + wi) * kKv8Block;                 // this block's first position
+  const int lo = static_cast<int>(max(first - blk0, 0LL));                     // rows [lo, hi) are new
+  const int hi = static_cast<int>(min(end - blk0, static_cast<long long>(kKv8Block)));
+  if (lo >= hi) return;
+  const int lane = threadIdx.x % kLanes;
+  const int row0 = threadIdx.x / kLanes;
+  const long long bh = static_cast<long long>(b) * p.kv_heads + h;
+  const int n_blocks = (p.capacity + kKv8Block - 1) / kKv8Block;
+  float* scale = p.scale[kv] + bh * n_blocks + blk0 / kKv8Block;
+  uint8_t* codes = p.codes[kv] + (bh * p.capacity + blk0) * HD + lane * 8;
+  const __half* src = p.src[kv] + b * p.bat[kv] + h * p.head[kv] + (blk0 - start) * p.tok[kv] + lane * 8;
+  const float before = lo > 0 ? *scale : 0.f;
+  uint4 x[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = row0 + i * kRowsPerPass;
+    if (r >= lo && r < hi) x[i] = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+  }
+  __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = row0 + i * kRowsPerPass;
+    if (r >= lo && r < hi)
+      mx = __hmax2(mx, __hmax2(__hmax2(finite_abs(x[i].x), finite_abs(x[i].y)),
+                               __hmax2(finite_abs(x[i].z), finite_abs(x[i].w))));
+  }
+  float a = fmaxf(__low2float(mx), __high2float(mx));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWriteThreads / 32; ++i) a = fmaxf(a, warp_max[i]);
+  const float s = fmaxf(__fmul_rn(a, 1.f / kKv8Top<FMT>), before);
+  const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = row0 + i * kRowsPerPass;
+    if (r >= lo && r < hi) {
+      uint2 c = make_uint2(0u, 0u);
+      if (inv > 0.f) c = make_uint2(quantise4<FMT>(x[i].x, x[i].y, inv), quantise4<FMT>(x[i].z, x[i].w, inv));
+      *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD) = c;
+    }
+  }
+  if (threadIdx.x == 0) *scale = s;
+  if (lo > 0 && s > before) {
+    // Older tokens of the block under the larger scale.
+    const float f = __fmul_rn(before, inv);
+    for (int r = row0; r < lo; r += kRowsPerPass) {
+      uint2* at = reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD);
+      uint2 c = *at;
+      uint32_t* word[2] = {&c.x, &c.y};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t l, u;
+        kv8_to_half2<FMT>(*word[k], l, u);
+        const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&l));
+        const float2 fu = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        *word[k] = kv8_pack4<FMT>(__fmul_rn(fl.x, f), __fmul_rn(fl.y, f), __fmul_rn(fu.x, f), __fmul_rn(fu.y, f));
+      }
+      *at = c;
+    }
+  }
+}
+
+constexpr int kReadThreads = 256;
+
+// One CTA per (64 positions, head, sequence, K or V); a thread turns 8 codes
+// into 16 bytes, several rows in flight.
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadParams p, int chunks) {
+  constexpr int kLanes = HD / 8;
+  constexpr int kRowsPerPass = kReadThreads / kLanes;
+  constexpr int kPasses = kKv8Block / kRowsPerPass;
+  int w = blockIdx.x;
+  const int kv = w & 1;
+  w >>= 1;
+  const int h = w % p.kv_heads;
+  w /= p.kv_heads;
+  const int b = w / chunks;
+  const int t0 = w % chunks * kKv8Block;
+  const int len = p.lens != nullptr ? p.lens[b] : p.capacity;
+  const int lane = threadIdx.x % kLanes;
+  const long long bh = static_cast<long long>(b) * p.kv_heads + h;
+  const int n_blocks = (p.capacity + kKv8Block - 1) / kKv8Block;
+  const float* scale = (kv ? p.scale[1] : p.scale[0]) + bh * n_blocks;
+  const uint8_t* codes = (kv ? p.codes[1] : p.codes[0]) + bh * p.capacity * HD + lane * 8;
+  __half* out = (kv ? p.out[1] : p.out[0]) + b * p.bat + h * p.head + lane * 8;
+  uint2 c[kPasses];
+  float s[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = t0 + threadIdx.x / kLanes + i * kRowsPerPass;
+    const int pos = p.start + t;
+    c[i] = make_uint2(0u, 0u);
+    s[i] = 0.f;
+    if (t < p.tokens && pos < len) {
+      c[i] = __ldg(reinterpret_cast<const uint2*>(codes + static_cast<long long>(pos) * HD));
+      s[i] = __ldg(scale + pos / kKv8Block);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = t0 + threadIdx.x / kLanes + i * kRowsPerPass;
+    if (t < p.tokens) {
+      uint32_t r[4];
+      const uint32_t word[2] = {c[i].x, c[i].y};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t l, u;
+        kv8_to_half2<FMT>(word[k], l, u);
+        const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&l));
+        const float2 fu = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        const __half2 hl = __floats2half2_rn(fl.x * s[i], fl.y * s[i]);
+        const __half2 hu = __floats2half2_rn(fu.x * s[i], fu.y * s[i]);
+        r[2 * k] = *reinterpret_cast<const uint32_t*>(&hl);
+        r[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hu);
+      }
+      *reinterpret_cast<uint4*>(out + static_cast<long long>(t) * p.tok) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream) {
+  // Blocks that `tokens` tokens from any start can touch.
+  const int window = (p.tokens + kKv8Block - 2) / kKv8Block + 1;
+  const long long ctas = 2LL * window * p.batch * p.kv_heads;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kernel = p.format == kKv8Int8
+                    ? (p.head_dim == 128 ? kv8_write_kernel<kKv8Int8, 128> : kv8_write_kernel<kKv8Int8, 64>)
+                    : (p.head_dim == 128 ? kv8_write_kernel<kKv8E4m3, 128> : kv8_write_kernel<kKv8E4m3, 64>);
+  kernel<<<static_cast<unsigned>(ctas), kWriteThreads, 0, stream>>>(p, window);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv8_read(const Kv8ReadParams& p, cudaStream_t stream) {
+  const int chunks = (p.tokens + kKv8Block - 1) / kKv8Block;
+  const long long ctas = 2LL * chunks * p.batch * p.kv_heads;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kernel = p.format == kKv8Int8
+                    ? (p.head_dim == 128 ? kv8_read_kernel<kKv8Int8, 128> : kv8_read_kernel<kKv8Int8, 64>)
+                    : (p.head_dim == 128 ? kv8_read_kernel<kKv8E4m3, 128> : kv8_read_kernel<kKv8E4m3, 64>);
+  kernel<<<static_cast<unsigned>(ctas), kReadThreads, 0, stream>>>(p, chunks);
+  return cudaGetLastError();
+}
+
+}  // namespace ax

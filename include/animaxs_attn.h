@@ -41,8 +41,9 @@ extern "C" {
 /* 2: animaxs_proj_desc gained the weight-storage fields (w_storage, w_scale,
  * w_zero, w_packed_stride); the peer-group and dequant entry points.
  * 3: animaxs_attn_desc gained `numerics`; the cross-K/V cache, weight
- * streamer and no-alloc status entry points. */
-#define ANIMAXS_ATTN_ABI_VERSION 3
+ * streamer and no-alloc status entry points.
+ * 4: the 8-bit K/V cache (animaxs_kv8_*). */
+#define ANIMAXS_ATTN_ABI_VERSION 4
 
 /* Status codes.  The reference throws AnimapkError.validation(String) for every
  * argument problem (AttentionExecutor.swift:778-825) and surfaces GPU errors as
@@ -312,6 +313,93 @@ int animaxs_cross_kv_cache_block(const animaxs_cross_kv_cache* cache, int block,
  * marks every block not ready. */
 int animaxs_cross_kv_cache_mark_ready(animaxs_cross_kv_cache* cache, int block, int ready);
 int animaxs_cross_kv_cache_reset(animaxs_cross_kv_cache* cache);
+
+/* ---- 8-bit K/V cache ---------------------------------------------------------
+ * A K/V cache in half the memory of fp16, written as tokens arrive, read back,
+ * and attended to directly.  No counterpart exists in the reference, whose
+ * caches are fp16 (CrossKVCache, DiTBlockExecutor.swift:19-43); it serves the
+ * same callers: the cross-attention K/V of every block, written once per
+ * generation, and a text encoder's cache that grows token by token.
+ *
+ * A cache is a view of four device buffers that the caller owns:
+ *   k_codes, v_codes  [batch][kv_heads][capacity][head_dim], one byte a value
+ *   k_scale, v_scale  fp32 [batch][kv_heads][ceil(capacity / 64)]
+ * A value is code * scale of its head and 64-token block.  INT8 codes are
+ * -127..127, E4M3 codes are 8-bit floats of magnitude <= 448.  The caller keeps
+ * each sequence's length; what lies at or past it is never read, so neither
+ * codes nor scales have to be initialised. */
+typedef enum animaxs_kv8_format { ANIMAXS_KV8_INT8 = 0, ANIMAXS_KV8_E4M3 = 1 } animaxs_kv8_format;
+
+#define ANIMAXS_KV8_BLOCK_TOKENS 64 /* tokens that share a scale */
+
+typedef struct animaxs_kv8_cache {
+  int32_t batch, capacity, kv_heads;
+  int32_t head_dim; /* 64 or 128 */
+  int32_t format;   /* animaxs_kv8_format */
+  void* k_codes;    /* 16-byte aligned */
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+} animaxs_kv8_cache;
+
+/* Bytes of one of the two code buffers and of one of the two scale buffers. */
+int animaxs_kv8_cache_bytes(int batch, int capacity, int kv_heads, int head_dim, int64_t* code_bytes,
+                            int64_t* scale_bytes);
+
+/* New tokens of every sequence: token t of sequence b goes to position
+ * start_b + t.  Strides are in fp16 elements, multiples of 8. */
+typedef struct animaxs_kv8_write_desc {
+  int32_t tokens;        /* rows in k and v per sequence (>= 1) */
+  int32_t start;         /* position of token 0 */
+  const int32_t* starts; /* optional DEVICE int32[batch]; overrides start per sequence */
+  const int32_t* counts; /* optional DEVICE int32[batch]: only the first counts[b] tokens are written */
+  int64_t k_tok_stride, k_head_stride, k_batch_stride;
+  int64_t v_tok_stride, v_head_stride, v_batch_stride;
+} animaxs_kv8_write_desc;
+
+/* Quantise fp16 k and v ([batch][tokens][kv_heads][head_dim], any strides)
+ * into the cache.  For each head and 64-token block that gets new tokens, with
+ * a the largest finite magnitude among them and M = 127 or 448:
+ *   s = a * (1 / M), and if the block holds tokens before the sequence's start
+ *   position, s = max(s, the block's scale); where that raises the scale,
+ *   those tokens' codes become round(code * (old scale * (1 / s)));
+ *   new codes are round(x * (1 / s)), all zero when s is 0.
+ * Arithmetic is fp32, rounding to nearest even.  NaN is stored as 0 and an
+ * infinity as +-M.  Positions outside [0, capacity) are not written.  A write
+ * ends the sequence: tokens behind the last new one in its block no longer
+ * have a scale of their own.  Repeating a write changes nothing. */
+int animaxs_kv8_write(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
+                      const animaxs_kv8_write_desc* desc, const void* k, const void* v, void* stream);
+
+/* Read positions [start, start + tokens) back as fp16, code * scale rounded
+ * once, into k_out and v_out ([batch][tokens][kv_heads][head_dim], one set of
+ * element strides for both).  `lens` (optional DEVICE int32[batch]): rows at
+ * or past position lens[b] are stored as zeros. */
+int animaxs_kv8_read(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache, int start, int tokens,
+                     const int32_t* lens, void* k_out, void* v_out, int64_t tok_stride, int64_t head_stride,
+                     int64_t batch_stride, void* stream);
+
+/* Attention of fp16 q over the cache, fp16 output:
+ *   o = softmax(scale * q . (code_k * scale_k) + mask) (code_v * scale_v).
+ * Of `desc` it takes batch, heads, kv_heads, q_len, head_dim, the q and o
+ * strides and extents, scale, kv_len (the most tokens of any sequence, <=
+ * capacity), kv_valid_len and kv_valid_lens (each sequence's length; zero in
+ * kv_valid_lens is a sequence without tokens), causal, and qk_norm RMS with
+ * qk_norm_targets Q_ONLY (K is normalised before it is written).  The k and v
+ * strides are not used.  q_len and kv_len are independent; with causal, query
+ * token i stands at position length - q_len + i and sees the keys up to its
+ * own.  A query that sees no key gets zeros.  Scores, softmax statistics and
+ * accumulators are fp32, probabilities enter the second product as fp16.
+ * Head dims 64 and 128, numerics LEGACY; with a score probe set the call
+ * returns ANIMAXS_ERR_UNSUPPORTED. */
+int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
+                             const animaxs_attn_desc* desc, const void* q, void* o, void* stream);
+
+/* Validate exactly as the calls above do, without a GPU. */
+int animaxs_kv8_write_validate(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
+                               const animaxs_kv8_write_desc* desc, const void* k, const void* v);
+int animaxs_kv8_attn_validate(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
+                              const animaxs_attn_desc* desc, const void* q, const void* o);
 
 /* ---- Weight streaming --------------------------------------------------------
  * Replaces WeightStreamer (WeightStreamer.swift:84-213): bounded device memory
