@@ -21,7 +21,7 @@ CALL_BENCH = os.path.join(BUILD, "call_bench")
 SOURCES = ["attn_api.cu", "attn_fwd_sm100.cu", "attn_s3_sm100.cu", "attn_wide_sm100.cu", "qk_norm.cu", "sharded.cu",
            "noalloc.cu", "proj_api.cu", "proj_sm100.cu", "dequant_sm100.cu",
            "peer_sync.cu", "peer_sharded.cu", "cross_kv_cache.cu", "weight_streamer.cu",
-           "kv8_api.cu", "kv8_cache.cu", "kv8_rows_sm100.cu"]
+           "kv8_api.cu", "kv8_cache.cu", "kv8_rows_sm100.cu", "kv8_attn_sm100.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3,-Wall",
          "--expt-relaxed-constexpr", "-Xptxas", "-v"]
@@ -55,6 +55,28 @@ REGISTER_SPLITS = {
     "attn_fwd_sm100.cu": ("attn_fwd_sm100_kernel", "AX_SOFTMAX_REGS", "AX_OTHER_REGS", "kSoftmaxThreads"),
     "proj_sm100.cu": ("proj_sm100_kernel", "AX_EPI_REGS", "AX_PROJ_OTHER_REGS", "kEpiThreads"),
 }
+
+# A three-way split: source file -> (kernel-name pattern, [(count define, threads)]).
+REGISTER_SHARES = {
+    "kv8_attn_sm100.cu": ("kv8_attn_sm100_kernel", [("AX_KV8_SOFTMAX_REGS", 256), ("AX_KV8_CONVERT_REGS", 128),
+                                                    ("AX_KV8_OTHER_REGS", 128)]),
+}
+
+
+def check_register_shares(source: str, ptxas_log: str) -> None:
+    """check_register_split for a kernel whose warpgroups have more than two counts."""
+    import re
+    kernel, shares = REGISTER_SHARES[os.path.basename(source)]
+    text = open(source).read()
+    regs = [(int(re.search(rf"#define {name} (\d+)", text).group(1)), n) for name, n in shares]
+    counts = re.findall(rf"entry function '[^']*{kernel}[^']*'.*?Used (\d+) registers", ptxas_log, re.S)
+    if not counts:
+        raise RuntimeError(f"could not read {kernel}'s register count from ptxas")
+    need, threads = sum(r * n for r, n in regs), sum(n for _, n in regs)
+    for launch in map(int, counts):
+        if need > threads * launch or any(r % 8 for r, _ in regs):
+            raise RuntimeError(f"{kernel}: register shares {regs} = {need} exceed the launch allocation "
+                               f"{threads}x{launch} = {threads * launch}")
 
 
 def check_register_split(source: str, ptxas_log: str) -> None:
@@ -105,6 +127,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for cmd, res in logs:
         if os.path.basename(cmd[-3]) in REGISTER_SPLITS:
             check_register_split(cmd[-3], res.stderr)
+        if os.path.basename(cmd[-3]) in REGISTER_SHARES:
+            check_register_shares(cmd[-3], res.stderr)
     if force or jobs or not _newer(LIB, objs):
         link = [cc, *ARCH, "-shared", "-o", LIB + ".tmp", *objs, "-ldl", "-Xcompiler", "-fPIC"]
         res = subprocess.run(link, capture_output=True, text=True)

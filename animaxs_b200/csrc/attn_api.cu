@@ -316,6 +316,31 @@ int ax_make_tmap_codes(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base
   return ANIMAXS_OK;
 }
 
+int ax_make_tmap_rows(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t pack,
+                      int64_t tokens, int64_t lines, int64_t batch, int64_t st, int64_t sh, int64_t sb) {
+  auto fn = encode_fn();
+  if (fn == nullptr)
+    return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  // As in ax_make_tmap, a dimension of extent 1 gets any legal stride; a batch
+  // of one shared q is a batch of extent 1.
+  if (sb == 0) batch = 1;
+  const int64_t any = dim * 2;
+  cuuint64_t dims[5] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(pack), static_cast<cuuint64_t>(tokens),
+                        static_cast<cuuint64_t>(lines), static_cast<cuuint64_t>(batch)};
+  cuuint64_t strides[4] = {static_cast<cuuint64_t>(pack > 1 ? sh * 2 : any),
+                           static_cast<cuuint64_t>(tokens > 1 ? st * 2 : any),
+                           static_cast<cuuint64_t>(lines > 1 ? sh * pack * 2 : any),
+                           static_cast<cuuint64_t>(batch > 1 ? sb * 2 : any)};
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(pack), static_cast<cuuint32_t>(128 / pack), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return ANIMAXS_OK;
+}
+
 // ------------------------------------------------------------------ forward --
 extern "C" int animaxs_attn_scratch_bytes(const animaxs_attn_desc* d, int64_t* bytes) {
   if (d == nullptr || bytes == nullptr) return ANIMAXS_ERR_INVALID_ARG;

@@ -287,7 +287,6 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   p.v_scale = cache->v_scale;
   p.status = ctx->d_status;
   p.rows = p.group * p.q_len;
-  p.row_tiles = (p.rows + 15) / 16;
   if (d->qk_norm == ANIMAXS_QK_RMS) {
     // q normalised into context scratch, by the kernel that normalises for animaxs_attn_forward.
     rc = ax_ensure_scratch(ctx, static_cast<size_t>(d->batch) * d->q_len * d->heads * D * 2);
@@ -318,17 +317,34 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
     p.q_head = j.out_head;
     p.q_batch = j.out_batch;
   }
-  CUtensorMap tk, tv;
+  // Up to 16 rows of a kv head fit the row kernel's one tile, which streams the
+  // cache once; more rows are bound by the products and go to the tensor cores.
+  const bool few = p.rows <= 16;
+  CUtensorMap tq, tk, tv;
   const int64_t heads = static_cast<int64_t>(cache->batch) * cache->kv_heads;
-  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, ax::kKv8Block);
-  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, ax::kKv8Block);
+  const int box = few ? ax::kKv8Block : ax::kTileN;
+  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, box);
+  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, box);
   if (rc != ANIMAXS_OK) return rc;
-  const int grid = ax::kv8_rows_grid(p, ctx->num_sms);
-  rc = ensure_split(ctx, ax::kv8_rows_part_floats(d->head_dim, grid), static_cast<size_t>(heads) * p.row_tiles);
-  if (rc != ANIMAXS_OK) return rc;
-  p.part = ctx->kv8_part;
-  p.count = ctx->kv8_count;
-  const cudaError_t e = ax::launch_kv8_rows(tk, tv, p, grid, ctx->device, s);
+  cudaError_t e;
+  if (few) {
+    p.row_tiles = 1;
+    const int grid = ax::kv8_rows_grid(p, ctx->num_sms);
+    rc = ensure_split(ctx, ax::kv8_rows_part_floats(d->head_dim, grid), static_cast<size_t>(heads));
+    if (rc != ANIMAXS_OK) return rc;
+    p.part = ctx->kv8_part;
+    p.count = ctx->kv8_count;
+    e = ax::launch_kv8_rows(tk, tv, p, grid, ctx->device, s);
+  } else {
+    if (!ax::kv8_attn_plan(&p, ctx->num_sms))
+      return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "attention byte size overflow");
+    rc = ensure_split(ctx, ax::kv8_attn_part_floats(p), 0);
+    if (rc != ANIMAXS_OK) return rc;
+    p.part = ctx->kv8_part;
+    rc = ax_make_tmap_rows(ctx, &tq, p.q, D, p.pack, p.q_len, p.lines, p.batch, p.q_tok, p.q_head, p.q_batch);
+    if (rc != ANIMAXS_OK) return rc;
+    e = ax::launch_kv8_attn(tq, tk, tv, p, ctx->num_sms, ctx->device, s);
+  }
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "attention launch");
   ctx->last_error.clear();
   return ANIMAXS_OK;

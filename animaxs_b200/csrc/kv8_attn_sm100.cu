@@ -1,0 +1,665 @@
+// kv8_attn_sm100.cu -- attention of many query rows over the 8-bit K/V cache:
+// cross attention of an image's tokens to a cached context, prompt chunks.
+//
+// The mathematics is that of kv8_rows_sm100.cu (the blocks' scales folded into
+// the exponent); the products run on the tensor cores as 128-row tcgen05
+// tiles.  Those take fp16 operands from shared memory, so four warps turn each
+// tile of 128 keys from codes into the fp16 layout the MMAs read, exactly, as
+// it arrives; two 128-row query tiles share every converted tile.
+//
+// Rows: with a power-of-two group the rows of a kv head are its query tokens x
+// the group's heads (row = token * group + head), so that short chunks fill a
+// tile; otherwise every query head is on its own.
+//
+// A work item is a pair of query tiles (A, B) of one (sequence, head line) and,
+// when the pairs alone would leave SMs idle, one of n_split parts of their
+// keys; kv8_join_kernel then joins the parts in order.  Items are dealt
+// round-robin to one persistent CTA per SM.  Sixteen warps:
+//   0-3, 4-7   softmax of tile A / B: thread t owns row t (= TMEM lane t)
+//   8-11       conversion: thread t turns key row t of each K and V tile
+//   12         MMA issuer and TMEM owner
+//   13         TMA producer: Q tiles; code tiles K_0, V_0, K_1, V_1, ... into a 2-slot ring
+//   14-15      idle (they complete the warpgroup)
+// TMEM (512 columns): S_A [0,128), S_B [128,256) (P_X overlays the first 64
+// columns of S_X), O_A [256,..), O_B.  The tensor core alternates PV_A(j),
+// QK_A(j+1), PV_B(j), QK_B(j+1), P is published in halves of 64 keys, and O
+// is rescaled only when a row's maximum grows by more than 2^8.
+// Every wait is bounded; a timeout raises the CTA's abort flag and the status
+// bit, and the CTA drains and exits.
+#include <atomic>
+
+#include "api_internal.h"
+#include "flash_common.cuh"
+#include "kernels.h"
+#include "kv8_common.cuh"
+
+namespace ax {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRaw = 2, kStages = 2;
+template <int HD>
+struct Smem {
+  static constexpr uint32_t kTile = kTileM * HD * 2;     // fp16 tile of 128 rows
+  static constexpr uint32_t kCodes = kTileN * HD;        // code tile of 128 keys
+  static constexpr uint32_t kQ = 0;                      // Q_A, Q_B
+  static constexpr uint32_t kK = kQ + 2 * kTile;
+  static constexpr uint32_t kV = kK + kStages * kTile;
+  static constexpr uint32_t kRing = kV + kStages * kTile;
+  static constexpr uint32_t kBar = kRing + kRaw * kCodes;
+  static constexpr uint32_t kBytes = kBar + 512 + 1024;  // + alignment slack
+};
+static_assert(Smem<128>::kBytes <= 227 * 1024, "shared memory exceeds the 227 KiB opt-in");
+
+enum : int {
+  kBarQ = 0,
+  kBarRawFull,                             // +slot
+  kBarRawEmpty = kBarRawFull + kRaw,       // +slot (4 warp arrivals)
+  kBarKFull = kBarRawEmpty + kRaw,         // +stage (4 warp arrivals)
+  kBarKEmpty = kBarKFull + kStages,        // +stage
+  kBarVFull = kBarKEmpty + kStages,        // +stage (4 warp arrivals)
+  kBarVEmpty = kBarVFull + kStages,        // +stage
+  kBarSFull = kBarVEmpty + kStages,        // +tile
+  kBarPHalf = kBarSFull + 2,               // +2*tile + half (128 arrivals)
+  kBarODone = kBarPHalf + 4,               // +tile
+  kBarQFree = kBarODone + 2,
+  kBarDone,
+  kNumBars
+};
+constexpr uint32_t kSlotTmem = kNumBars * 8;
+constexpr uint32_t kSlotAbort = kSlotTmem + 4;
+// Per key tile and 64-key block: factor of the scores, log2 scale_v, 1 / scale_v
+// (float4 [4 tiles][2 blocks]).  Four tiles deep: K tile g is converted after
+// QK(g-2) retired, which follows the softmax's use of tile g-3.
+constexpr uint32_t kSlotScale = 256;
+static_assert(kSlotAbort + 4 <= kSlotScale && kSlotScale + 4 * 2 * 16 <= 512, "barrier block overflows");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 256;
+constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
+
+// Register split (setmaxnreg) of the 512 x 128 registers of the launch: softmax
+// 2 x 128 threads, conversion 128, MMA / TMA 128 (build.py checks the sum).
+#define AX_KV8_SOFTMAX_REGS 208
+#define AX_KV8_CONVERT_REGS 56
+#define AX_KV8_OTHER_REGS 40
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+struct Item {
+  int q0, h, b, kvh, len;
+  int j0;          // first key tile
+  int nA, nB, n;   // key tiles of A, of B, of the item
+};
+
+__device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
+  Item it;
+  const int s = w % p.n_split;
+  w /= p.n_split;
+  const int pair = p.causal ? p.pairs - 1 - w % p.pairs : w % p.pairs;  // the longest first
+  w /= p.pairs;
+  it.h = w % p.lines;
+  it.b = w / p.lines;
+  it.kvh = p.pack == p.group ? it.h : it.h / p.group;
+  it.q0 = pair * 2 * kTileM;
+  it.len = kv8_len(p.lens, p.kv_valid, p.kv_len, it.b);
+  auto tiles = [&](int r0) {
+    if (r0 >= p.rows) return 0;
+    int e = it.len;
+    if (p.causal) e = min(e, max(it.len - p.q_len + min(r0 + kTileM - 1, p.rows - 1) / p.pack + 1, 0));
+    return (e + kTileN - 1) / kTileN;
+  };
+  const int a = tiles(it.q0), b = tiles(it.q0 + kTileM);
+  const int n = max(a, b);
+  it.j0 = static_cast<int>(static_cast<long long>(n) * s / p.n_split);
+  const int j1 = static_cast<int>(static_cast<long long>(n) * (s + 1) / p.n_split);
+  it.nA = max(min(a, j1) - it.j0, 0);
+  it.nB = max(min(b, j1) - it.j0, 0);
+  it.n = j1 - it.j0;
+  return it;
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv8_attn_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                          const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  using L = Smem<HD>;
+  const uint32_t sQ = base + L::kQ, sK = base + L::kK, sV = base + L::kV, sR = base + L::kRing;
+  const uint32_t bar0 = base + L::kBar;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kBar + kSlotTmem);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kBar + kSlotAbort);
+#define BAR(i) (bar0 + 8u * static_cast<uint32_t>(i))
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int w0 = static_cast<int>(blockIdx.x);
+  const int wstep = static_cast<int>(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNumBars; ++i) {
+      uint32_t count = 1;
+      if (i >= kBarRawEmpty && i < kBarRawEmpty + kRaw) count = 4;
+      if (i >= kBarKFull && i < kBarKFull + kStages) count = 4;
+      if (i >= kBarVFull && i < kBarVFull + kStages) count = 4;
+      if (i >= kBarPHalf && i < kBarPHalf + 4) count = 128;
+      mbar_init(BAR(i), count);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(bar0 + kSlotTmem, kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 13 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AX_KV8_OTHER_REGS));
+    if (warp == 13) {
+      // ---------------------------------------------------------- producer --
+      if (lane == 0) {
+        int armed_q = 0, armed[kRaw] = {};
+        uint32_t g = 0;  // code tiles loaded so far
+        auto load = [&](const CUtensorMap* tm, int row0, int head) -> bool {
+          const uint32_t slot = g % kRaw;
+          if (!mbar_wait(BAR(kBarRawEmpty + slot), ((g / kRaw) & 1u) ^ 1u, abort_flag, p.status)) return false;
+          mbar_arrive_expect_tx(BAR(kBarRawFull + slot), L::kCodes);
+          tma_load_3d(sR + slot * L::kCodes, tm, BAR(kBarRawFull + slot), 0, row0, head);
+          ++armed[slot];
+          ++g;
+          return true;
+        };
+        bool ok = true;
+        int it = 0;
+        for (int w = w0; ok && w < p.n_items; w += wstep) {
+          const Item I = kv8_item(p, w);
+          if (I.n == 0) continue;
+          // Q is reloaded once the previous item's last QK has retired.
+          if (it > 0 && !(ok = mbar_wait(BAR(kBarQFree), static_cast<uint32_t>((it - 1) & 1), abort_flag, p.status)))
+            break;
+          const int first = I.nA > 0 ? 0 : 1, last = I.nB > 0 ? 1 : 0;
+          mbar_arrive_expect_tx(BAR(kBarQ), (last - first + 1) * L::kTile);
+          for (int x = first; x <= last; ++x)
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+              tma_load_5d(sQ + x * L::kTile + c * kPanelBytes, &tm_q, BAR(kBarQ), 64 * c, 0,
+                          (I.q0 + x * kTileM) / p.pack, I.h, p.q_batch != 0 ? I.b : 0);
+          ++armed_q;
+          ++it;
+          const int head = I.b * p.kv_heads + I.kvh;
+          for (int j = 0; ok && j < I.n; ++j) {
+            if (!(ok = load(&tm_k, (I.j0 + j) * kTileN, head))) break;
+            ok = load(&tm_v, (I.j0 + j) * kTileN, head);
+          }
+        }
+        // Never leave the CTA with a tensor copy still landing in shared memory.
+        if (armed_q) mbar_wait_drain(BAR(kBarQ), (armed_q - 1) & 1);
+        for (int s = 0; s < kRaw; ++s)
+          if (armed[s]) mbar_wait_drain(BAR(kBarRawFull + s), (armed[s] - 1) & 1);
+      }
+    } else if (warp == 12) {
+      // --------------------------------------------------------------- MMA --
+      const uint32_t sQA = sQ, sQB = sQ + L::kTile;
+      uint32_t gk = 0, gv = 0;  // K / V tiles consumed so far
+      uint32_t tA = 0, tB = 0;  // tiles of A / B in earlier items (PHalf phases)
+      bool ok = true;
+      uint32_t it = 0;
+      auto k_full = [&](uint32_t g) {
+        return mbar_wait_warp(BAR(kBarKFull + g % kStages), (g / kStages) & 1u, abort_flag, p.status);
+      };
+      for (int w = w0; ok && w < p.n_items; w += wstep) {
+        const Item I = kv8_item(p, w);
+        const int nA = I.nA, nB = I.nB, n_kv = I.n;
+        if (n_kv == 0) continue;
+        if (!(ok = mbar_wait_warp(BAR(kBarQ), it & 1u, abort_flag, p.status))) break;
+        ++it;
+        if (!(ok = k_full(gk))) break;
+        tc_fence_after();
+        const uint32_t k0 = sK + (gk % kStages) * L::kTile;
+        if (nA > 0) {
+          issue_qk<HD>(tmem + 0, sQA, k0);
+          tc_commit_warp(BAR(kBarSFull + 0));
+        }
+        if (nB > 0) {
+          issue_qk<HD>(tmem + 128, sQB, k0);
+          tc_commit_warp(BAR(kBarSFull + 1));
+        }
+        tc_commit_warp(BAR(kBarKEmpty + gk % kStages));
+        ++gk;
+        if (n_kv == 1) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
+        for (int j = 0; j < n_kv; ++j) {
+          const uint32_t vst = gv % kStages;
+          const int j1 = j + 1;
+          const uint32_t vt = sV + vst * L::kTile;
+          const uint32_t kt1 = sK + (gk % kStages) * L::kTile;
+          if (!(ok = mbar_wait_warp(BAR(kBarVFull + vst), (gv / kStages) & 1u, abort_flag, p.status))) break;
+          if (j < nA) {
+            // The softmax threads publish an item's first P only after their
+            // previous epilogue has read O out of TMEM.
+            const uint32_t pph = (tA + j) & 1u;
+            if (!(ok = mbar_wait_warp(BAR(kBarPHalf + 0), pph, abort_flag, p.status))) break;
+            tc_fence_after();
+            issue_pv_half<HD, false>(tmem + kColO, tmem + 0, vt, 0, j > 0);
+            if (!(ok = mbar_wait_warp(BAR(kBarPHalf + 1), pph, abort_flag, p.status))) break;
+            tc_fence_after();
+            issue_pv_half<HD, false>(tmem + kColO, tmem + 0, vt, 1, true);
+            if (j == nA - 1) tc_commit_warp(BAR(kBarODone + 0));
+          }
+          if (j1 < n_kv) {
+            if (!(ok = k_full(gk))) break;
+            tc_fence_after();
+          }
+          if (j1 < nA) {
+            issue_qk<HD>(tmem + 0, sQA, kt1);
+            tc_commit_warp(BAR(kBarSFull + 0));
+          }
+          if (j < nB) {
+            const uint32_t pph = (tB + j) & 1u;
+            if (!(ok = mbar_wait_warp(BAR(kBarPHalf + 2), pph, abort_flag, p.status))) break;
+            tc_fence_after();
+            issue_pv_half<HD, false>(tmem + kColO + HD, tmem + 128, vt, 0, j > 0);
+            if (!(ok = mbar_wait_warp(BAR(kBarPHalf + 3), pph, abort_flag, p.status))) break;
+            tc_fence_after();
+            issue_pv_half<HD, false>(tmem + kColO + HD, tmem + 128, vt, 1, true);
+            if (j == nB - 1) tc_commit_warp(BAR(kBarODone + 1));
+          }
+          tc_commit_warp(BAR(kBarVEmpty + vst));  // V_j's last reader has been issued
+          ++gv;
+          if (j1 < nB) {
+            issue_qk<HD>(tmem + 128, sQB, kt1);
+            tc_commit_warp(BAR(kBarSFull + 1));
+          }
+          if (j1 < n_kv) {
+            tc_commit_warp(BAR(kBarKEmpty + gk % kStages));
+            ++gk;
+            if (j1 == n_kv - 1) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
+          }
+        }
+        tA += nA;
+        tB += nB;
+      }
+      // All MMAs this warp issued must retire before TMEM is released.
+      tc_commit_warp(BAR(kBarDone));
+      mbar_wait_drain(BAR(kBarDone), 0);
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AX_KV8_CONVERT_REGS));
+    // ---------------------------------------------------------- conversion --
+    // Thread t turns row t (one key): 16-byte runs of 16 codes become two
+    // 16-byte units of the 64-column SW128 panels.  Eight lanes that share a
+    // phase hold eight consecutive rows, so loads and stores meet no bank twice.
+    const int t = threadIdx.x - 256;
+    uint32_t g = 0;  // code tiles taken so far: K and V alternate
+    bool ok = true;
+    float nk = 0.f, nv = 0.f;  // threads 0 and 1: scales of their block of the next K tile
+    auto scales = [&](const Item& I, int j) {
+      const int blk = 2 * (I.j0 + j) + t;
+      // A block past the length has no scale.
+      const bool live = blk * kKv8Block < I.len;
+      const long long at = (static_cast<long long>(I.b) * p.kv_heads + I.kvh) * p.n_blocks + blk;
+      nk = live ? __ldg(p.k_scale + at) : 0.f;
+      nv = live ? __ldg(p.v_scale + at) : 0.f;
+    };
+    for (int w = w0; ok && w < p.n_items; w += wstep) {
+      const Item I = kv8_item(p, w);
+      if (t < 2 && I.n > 0) scales(I, 0);
+      for (int jj = 0; ok && jj < 2 * I.n; ++jj, ++g) {
+        const uint32_t slot = g % kRaw, st = (g >> 1) % kStages, use = (g >> 1) / kStages;
+        const bool is_v = (g & 1u) != 0;
+        ok = mbar_wait_warp(BAR(kBarRawFull + slot), (g / kRaw) & 1u, abort_flag, p.status);
+        if (!ok) break;
+        const uint32_t src = sR + slot * L::kCodes + t * HD;
+        uint4 c[HD / 16];
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const int at = HD == 128 ? i ^ (t & 7) : i ^ ((t >> 1) & 3);
+          c[i] = ld_shared_v4u(src + at * 16);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(kBarRawEmpty + slot));
+        // What lies past the length may decode to NaN: such keys become zeros.
+        if ((I.j0 + (jj >> 1)) * kTileN + t >= I.len) {
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        ok = mbar_wait_warp(BAR((is_v ? kBarVEmpty : kBarKEmpty) + st), (use & 1u) ^ 1u, abort_flag, p.status);
+        if (!ok) break;
+        const uint32_t dst = (is_v ? sV : sK) + st * L::kTile + t * 128;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          uint32_t h[8];
+          kv8_to_half2<FMT>(c[i].x, h[0], h[1]);
+          kv8_to_half2<FMT>(c[i].y, h[2], h[3]);
+          kv8_to_half2<FMT>(c[i].z, h[4], h[5]);
+          kv8_to_half2<FMT>(c[i].w, h[6], h[7]);
+          const uint32_t panel = dst + (i >> 2) * kPanelBytes;
+          const int u = (i & 3) * 2;
+          st_shared_v4(panel + ((u ^ (t & 7)) << 4), h[0], h[1], h[2], h[3]);
+          st_shared_v4(panel + (((u + 1) ^ (t & 7)) << 4), h[4], h[5], h[6], h[7]);
+        }
+        if (!is_v && t < 2) {
+          // A block whose K scale is 0 has only zero codes: any factor gives its
+          // scores, 0; 1 keeps a masked -inf from meeting 0.
+          st_shared_v4(base + L::kBar + kSlotScale + ((g >> 1) & 3) * 32 + t * 16,
+                       __float_as_uint(nk > 0.f ? nk * p.scale_log2 : 1.f),
+                       __float_as_uint(nv > 0.f ? __log2f(nv) : kNoScale),
+                       __float_as_uint(nv > 0.f ? __fdividef(1.f, nv) : 8589934592.f), 0u);  // 2^33
+          if (jj + 2 < 2 * I.n) scales(I, (jj >> 1) + 1);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR((is_v ? kBarVFull : kBarKFull) + st));
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AX_KV8_SOFTMAX_REGS));
+    // ------------------------------------------------------------- softmax --
+    const int X = warp >> 2;          // 0: tile A, 1: tile B
+    const int t = threadIdx.x & 127;  // row within the tile == TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + X * 128;
+    const uint32_t o_addr = tmem + lane_base + kColO + X * HD;
+    bool ok = true;
+    uint32_t tX = 0;  // tiles of this query tile processed in earlier items
+    uint32_t gt = 0;  // key tiles of earlier items
+    uint32_t eX = 0;  // epilogues done in earlier items
+    for (int w = w0; ok && w < p.n_items; w += wstep) {
+      const Item I = kv8_item(p, w);
+      const int row = I.q0 + X * kTileM + t;
+      const int nX = X ? I.nB : I.nA;
+      const int tok = row / p.pack;
+      const int lim = p.causal ? min(I.len, I.len - p.q_len + tok + 1) : I.len;  // keys visible to this row
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nX; ++j) {
+        const int key0 = (I.j0 + j) * kTileN;
+        ok = mbar_wait(BAR(kBarSFull + X), (tX + j) & 1u, abort_flag, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+        tmem_ld32(s_addr + 0, s[0]);
+        tmem_ld32(s_addr + 32, s[1]);
+        tmem_ld32(s_addr + 64, s[2]);
+        tmem_ld32(s_addr + 96, s[3]);
+        tmem_ld_wait(s[0]);
+        asm volatile("" : AX_RW32(s[1])::"memory");
+        asm volatile("" : AX_RW32(s[2])::"memory");
+        asm volatile("" : AX_RW32(s[3])::"memory");
+        if (key0 + kTileN > lim) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (key0 + c >= lim) s[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+        }
+        float4 fac[2];  // factor, log2 scale_v, 1 / scale_v of the two blocks
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fac[i] = ld_shared_v4f(base + L::kBar + kSlotScale + ((gt + j) & 3) * 32 + i * 16);
+        // Row maximum of each 64-key block, then of s + log2 scale_v.
+#define SV(c) __uint_as_float(s[(c) >> 5][(c) & 31])
+        float top[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            mx[a] = fmax3(SV(64 * i + a), SV(64 * i + a + 4), SV(64 * i + a + 8));
+#pragma unroll
+            for (int c = 12; c < 60; c += 8) mx[a] = fmax3(mx[a], SV(64 * i + a + c), SV(64 * i + a + c + 4));
+            mx[a] = fmaxf(mx[a], SV(64 * i + a + 60));
+          }
+          top[i] = fmaf(fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]), fac[i].x, fac[i].y);
+        }
+#undef SV
+        const float m_new = fmax3(m, top[0], top[1]);
+        const bool grow = m_new > m + kRescaleThreshold;  // also true on the first tile with a visible key
+        const float alpha = grow ? ex2_approx(m - m_new) : 1.f;
+        if (grow) {
+          l *= alpha;
+          m = m_new;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+          // PV_X(j-1) precedes QK_X(j) in the MMA stream, so it has retired and O
+          // is stable; PV_X(j) starts only after this thread's first arrival below.
+#pragma unroll
+          for (int c4 = 0; c4 < HD / 32; ++c4) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c4 * 32, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_addr + c4 * 32, o);
+          }
+        }
+        const float base_m = (m == -INFINITY) ? 0.f : m;
+        uint32_t pk[2][32];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float2 mulv = make_float2(fac[half].x, fac[half].x);
+          const float off = fac[half].y - base_m;
+          const float2 offv = make_float2(off, off);
+          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int c = half * 64; c < half * 64 + 64; c += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(s[c >> 5][c & 31]),
+                                              __uint_as_float(s[c >> 5][(c + 1) & 31])),
+                                  mulv, offv);
+            float2 pr;
+            if (((c >> 1) & 7) < kPolyPairsPer8) {
+              pr = ex2_poly2(x);
+            } else {
+              pr.x = ex2_approx(x.x);
+              pr.y = ex2_approx(x.y);
+            }
+            acc[(c >> 1) & 1] = add2(acc[(c >> 1) & 1], pr);
+            pk[half][(c >> 1) & 31] = pack_half2(pr.x, pr.y);
+          }
+          // Publish this half of P: the MMA warp starts its half of PV_X(j)
+          // while the second half is still being computed.
+          tmem_st32(s_addr + half * 32, pk[half]);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(BAR(kBarPHalf + 2 * X + half));
+          const float2 a = add2(acc[0], acc[1]);
+          l = fmaf(a.x + a.y, fac[half].z, l);
+        }
+      }
+      if (!ok) break;
+      if (nX > 0) {
+        ok = mbar_wait(BAR(kBarODone + X), eX & 1u, abort_flag, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        ++eX;
+      }
+      tX += nX;
+      gt += I.n;
+      // A row without a visible key has m = -inf and l of masked entries only
+      // (2^-126 each); one with NaN scores has l = NaN.
+      const bool none = nX == 0 || (m == -INFINITY && l == l);
+      if (p.n_split > 1) {
+        // [item][tile][HD / 4][128 rows] float4, then m and l of the rows.
+        float* part = p.part + (2LL * w + X) * (kTileM * (HD + 2));
+        const bool live = row < p.rows;
+        if (live) {
+          part[kTileM * HD + t] = none ? -INFINITY : m;
+          part[kTileM * HD + kTileM + t] = none ? 0.f : l;
+        }
+        if (nX > 0) {
+#pragma unroll
+          for (int c4 = 0; c4 < HD / 32; ++c4) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c4 * 32, o);
+            tmem_ld_wait(o);
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                reinterpret_cast<uint4*>(part)[(c4 * 8 + i / 4) * kTileM + t] =
+                    make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+        }
+      } else {
+        const float inv_l = none ? 0.f : 1.f / l;
+        const int head = I.h * p.pack + row % p.pack;
+        __half* dst = p.o + I.b * p.o_batch + static_cast<long long>(tok) * p.o_tok + head * p.o_head;
+#pragma unroll
+        for (int c4 = 0; c4 < HD / 32; ++c4) {
+          uint32_t o[32];
+          if (nX > 0) {
+            tmem_ld32(o_addr + c4 * 32, o);
+            tmem_ld_wait(o);
+          }
+          if (row < p.rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (!none)
+                v = make_uint4(pack_half2(__uint_as_float(o[i]) * inv_l, __uint_as_float(o[i + 1]) * inv_l),
+                               pack_half2(__uint_as_float(o[i + 2]) * inv_l, __uint_as_float(o[i + 3]) * inv_l),
+                               pack_half2(__uint_as_float(o[i + 4]) * inv_l, __uint_as_float(o[i + 5]) * inv_l),
+                               pack_half2(__uint_as_float(o[i + 6]) * inv_l, __uint_as_float(o[i + 7]) * inv_l));
+              *reinterpret_cast<uint4*>(dst + c4 * 32 + i) = v;
+            }
+          }
+        }
+      }
+      tc_fence_before();  // O has been read before the next item's first P is published
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+#undef BAR
+}
+
+// Joins the n_split parts of every row in order: O = sum O'_s 2^(m_s - m) / sum l_s 2^(m_s - m).
+// A thread takes 8 output values of a row; consecutive threads take consecutive rows.
+template <int HD>
+__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
+  const int t = threadIdx.x;
+  const int d8 = blockIdx.x % (HD / 8);
+  int w = blockIdx.x / (HD / 8);  // (sequence, line, pair, tile)
+  const int X = w & 1;
+  w >>= 1;
+  const int pair = w % p.pairs;
+  const int row = pair * 2 * kTileM + X * kTileM + t;
+  if (row >= p.rows) return;
+  const int unit = w - pair + (p.causal ? p.pairs - 1 - pair : pair);  // as kv8_item numbers it
+  const int h = w / p.pairs % p.lines, b = w / p.pairs / p.lines;
+  float m = -INFINITY, l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+#pragma unroll 4
+  for (int s = 0; s < p.n_split; ++s) {
+    const float* part = p.part + (2LL * (static_cast<long long>(unit) * p.n_split + s) + X) * (kTileM * (HD + 2));
+    const float pm = __ldcg(part + kTileM * HD + t), pl = __ldcg(part + kTileM * HD + kTileM + t);
+    const float mn = fmaxf(m, pm);
+    const float fo = m == mn ? 1.f : ex2_approx(m - mn);
+    const float fn = pm == mn ? 1.f : ex2_approx(pm - mn);
+    m = mn;
+    l = l * fo + pl * fn;
+    if (pm == -INFINITY && pl == 0.f) continue;  // nothing stored (the first live part makes fo 0)
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8) * kTileM + t);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8 + 1) * kTileM + t);
+    a = make_float4(a.x * fo + x.x * fn, a.y * fo + x.y * fn, a.z * fo + x.z * fn, a.w * fo + x.w * fn);
+    c = make_float4(c.x * fo + y.x * fn, c.y * fo + y.y * fn, c.z * fo + y.z * fn, c.w * fo + y.w * fn);
+  }
+  const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
+  const int head = h * p.pack + row % p.pack;
+  *reinterpret_cast<uint4*>(p.o + b * p.o_batch + static_cast<long long>(row / p.pack) * p.o_tok + head * p.o_head +
+                            d8 * 8) =
+      make_uint4(pack_half2(a.x * inv, a.y * inv), pack_half2(a.z * inv, a.w * inv),
+                 pack_half2(c.x * inv, c.y * inv), pack_half2(c.z * inv, c.w * inv));
+}
+
+template <int FMT, int HD>
+cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p,
+                      int grid, int dev, cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  const uint64_t bit = 1ull << (dev & 63);
+  auto kernel = kv8_attn_sm100_kernel<FMT, HD>;
+  if ((configured.load(std::memory_order_acquire) & bit) == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kBytes);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  kernel<<<grid, kThreads, Smem<HD>::kBytes, stream>>>(tq, tk, tv, p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && p.n_split > 1) {
+    const int blocks = p.batch * p.lines * p.pairs * 2 * (HD / 8);
+    kv8_join_kernel<HD><<<blocks, 128, 0, stream>>>(p);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+
+// Fills in the rows, pairs and parts of a launch.  Parts: a pair of tiles over
+// all its keys is one item when the items fill the SMs; otherwise the keys are
+// cut into the number of parts for which the busiest SM has the least to do,
+// counting two key tiles' time for each item's start and end.
+bool kv8_attn_plan(Kv8AttnParams* p, int sms) {
+  p->pack = kTileM % p->group == 0 ? p->group : 1;
+  p->lines = p->kv_heads * p->group / p->pack;
+  p->rows = p->q_len * p->pack;
+  p->pairs = (p->rows + 2 * kTileM - 1) / (2 * kTileM);
+  const long long pairs = static_cast<long long>(p->batch) * p->lines * p->pairs;
+  const long long tiles = (p->kv_len + kTileN - 1) / kTileN;
+  p->n_split = 1;
+  if (pairs < sms) {
+    long long best = 0;
+    for (int s = 1; s <= 32 && s <= tiles; ++s) {
+      const long long cost = (pairs * s + sms - 1) / sms * ((tiles + s - 1) / s + 2);
+      if (s == 1 || cost < best) {
+        best = cost;
+        p->n_split = s;
+      }
+    }
+  }
+  if (pairs * p->n_split > 0x7fffffffLL / (2 * 16)) return false;
+  p->n_items = static_cast<int>(pairs * p->n_split);
+  return true;
+}
+size_t kv8_attn_part_floats(const Kv8AttnParams& p) {
+  return p.n_split > 1 ? 2 * static_cast<size_t>(p.n_items) * kTileM * (p.head_dim + 2) : 0;
+}
+
+cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                            const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream) {
+  const int grid = p.n_items < sms ? p.n_items : sms;
+  if (p.format == kKv8Int8)
+    return p.head_dim == 128 ? launch_hd<kKv8Int8, 128>(tq, tk, tv, p, grid, dev, stream)
+                             : launch_hd<kKv8Int8, 64>(tq, tk, tv, p, grid, dev, stream);
+  return p.head_dim == 128 ? launch_hd<kKv8E4m3, 128>(tq, tk, tv, p, grid, dev, stream)
+                           : launch_hd<kKv8E4m3, 64>(tq, tk, tv, p, grid, dev, stream);
+}
+
+}  // namespace ax
