@@ -19,7 +19,9 @@
 //   8-11       conversion: thread t turns key row t of each K and V tile
 //   12         MMA issuer and TMEM owner
 //   13         TMA producer: Q tiles; code tiles K_0, V_0, K_1, V_1, ... into a 2-slot ring
-//   14-15      idle (they complete the warpgroup)
+//   14         scheduler: works out the CTA's next items ahead of the other roles
+//              (divisions and the length's load, 2000 cycles when every role did it)
+//   15         idle (it completes the warpgroup)
 // TMEM (512 columns): S_A [0,128), S_B [128,256) (P_X overlays the first 64
 // columns of S_X), O_A [256,..), O_B.  The tensor core alternates PV_A(j),
 // QK_A(j+1), PV_B(j), QK_B(j+1), P is published in halves of 64 keys, and O
@@ -38,6 +40,8 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kRaw = 2, kStages = 2;
+constexpr int kItems = 2;  // items worked out ahead
+constexpr int kItemReaders = 14;
 template <int HD>
 struct Smem {
   static constexpr uint32_t kTile = kTileM * HD * 2;     // fp16 tile of 128 rows
@@ -60,10 +64,12 @@ enum : int {
   kBarVFull = kBarKEmpty + kStages,        // +stage (4 warp arrivals)
   kBarVEmpty = kBarVFull + kStages,        // +stage
   kBarSFull = kBarVEmpty + kStages,        // +tile
-  kBarPHalf = kBarSFull + 2,               // +2*tile + half (128 arrivals)
+  kBarPHalf = kBarSFull + 2,               // +2*tile + half (4 warp arrivals)
   kBarODone = kBarPHalf + 4,               // +tile
   kBarQFree = kBarODone + 2,
-  kBarDone,
+  kBarItemFull,                            // +entry
+  kBarItemEmpty = kBarItemFull + kItems,   // +entry (14 arrivals: every consuming warp)
+  kBarDone = kBarItemEmpty + kItems,
   kNumBars
 };
 constexpr uint32_t kSlotTmem = kNumBars * 8;
@@ -72,16 +78,17 @@ constexpr uint32_t kSlotAbort = kSlotTmem + 4;
 // (float4 [4 tiles][2 blocks]).  Four tiles deep: K tile g is converted after
 // QK(g-2) retired, which follows the softmax's use of tile g-3.
 constexpr uint32_t kSlotScale = 256;
-static_assert(kSlotAbort + 4 <= kSlotScale && kSlotScale + 4 * 2 * 16 <= 512, "barrier block overflows");
+constexpr uint32_t kSlotItem = kSlotScale + 4 * 2 * 16;  // Item [kItems]
+static_assert(kSlotAbort + 4 <= kSlotScale && kSlotItem + kItems * 48 <= 512, "barrier block overflows");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;
 constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
 // Register split (setmaxnreg) of the 512 x 128 registers of the launch: softmax
 // 2 x 128 threads, conversion 128, MMA / TMA 128 (build.py checks the sum).
-#define AX_KV8_SOFTMAX_REGS 208
-#define AX_KV8_CONVERT_REGS 56
-#define AX_KV8_OTHER_REGS 40
+#define AX_KV8_SOFTMAX_REGS 168
+#define AX_KV8_CONVERT_REGS 88
+#define AX_KV8_OTHER_REGS 88
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
@@ -99,14 +106,19 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
-struct Item {
-  int q0, h, b, kvh, len;
+struct alignas(16) Item {
+  int q0, h, b, kvh;
+  int len;
   int j0;          // first key tile
   int nA, nB, n;   // key tiles of A, of B, of the item
+  int w;           // its number, -1 past the last one
+  int pad[2];
 };
+static_assert(sizeof(Item) == 48, "items are read as three 16-byte words");
 
 __device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
   Item it;
+  it.w = w;
   const int s = w % p.n_split;
   w /= p.n_split;
   const int pair = p.causal ? p.pairs - 1 - w % p.pairs : w % p.pairs;  // the longest first
@@ -131,6 +143,7 @@ __device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
   it.n = j1 - it.j0;
   return it;
 }
+
 
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -157,7 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (i >= kBarRawEmpty && i < kBarRawEmpty + kRaw) count = 4;
       if (i >= kBarKFull && i < kBarKFull + kStages) count = 4;
       if (i >= kBarVFull && i < kBarVFull + kStages) count = 4;
-      if (i >= kBarPHalf && i < kBarPHalf + 4) count = 128;
+      if (i >= kBarPHalf && i < kBarPHalf + 4) count = 4;
+      if (i >= kBarItemEmpty && i < kBarItemEmpty + kItems) count = kItemReaders;
       mbar_init(BAR(i), count);
     }
     *abort_flag = 0;
@@ -177,6 +191,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // The CTA's next item (every consuming warp calls it once per item, converged
+  // or, for the producer, from its one active lane); w is -1 past the last one.
+  uint32_t items_read = 0;
+  auto next_item = [&](bool one_lane, bool& ok) {
+    const uint32_t e = items_read % kItems, ph = (items_read / kItems) & 1u;
+    ++items_read;
+    Item I;
+    I.w = -1;
+    ok = one_lane ? mbar_wait(BAR(kBarItemFull + e), ph, abort_flag, p.status)
+                  : mbar_wait_warp(BAR(kBarItemFull + e), ph, abort_flag, p.status);
+    if (!ok) return I;
+    const uint32_t at = base + L::kBar + kSlotItem + e * sizeof(Item);
+    const uint4 a = ld_shared_v4u(at), b = ld_shared_v4u(at + 16), c = ld_shared_v4u(at + 32);
+    I.q0 = a.x, I.h = a.y, I.b = a.z, I.kvh = a.w;
+    I.len = b.x, I.j0 = b.y, I.nA = b.z, I.nB = b.w;
+    I.n = c.x, I.w = c.y;
+    if (!one_lane) __syncwarp();
+    if (one_lane || lane == 0) mbar_arrive(BAR(kBarItemEmpty + e));
+    return I;
+  };
+
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AX_KV8_OTHER_REGS));
     if (warp == 13) {
@@ -195,10 +230,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         bool ok = true;
         int it = 0;
-        for (int w = w0; ok && w < p.n_items; w += wstep) {
-          const Item I = kv8_item(p, w);
+        while (true) {
+          const Item I = next_item(true, ok);
+          if (!ok || I.w < 0) break;
           if (I.n == 0) continue;
-          // Q is reloaded once the previous item's last QK has retired.
+          const int head = I.b * p.kv_heads + I.kvh;
+          // The first K and V tile before Q, whose buffer is still in use: they
+          // are converted while the previous item drains.
+          if (!(ok = load(&tm_k, I.j0 * kTileN, head))) break;
+          if (!(ok = load(&tm_v, I.j0 * kTileN, head))) break;
           if (it > 0 && !(ok = mbar_wait(BAR(kBarQFree), static_cast<uint32_t>((it - 1) & 1), abort_flag, p.status)))
             break;
           const int first = I.nA > 0 ? 0 : 1, last = I.nB > 0 ? 1 : 0;
@@ -210,11 +250,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                           (I.q0 + x * kTileM) / p.pack, I.h, p.q_batch != 0 ? I.b : 0);
           ++armed_q;
           ++it;
-          const int head = I.b * p.kv_heads + I.kvh;
-          for (int j = 0; ok && j < I.n; ++j) {
+          for (int j = 1; ok && j < I.n; ++j) {
             if (!(ok = load(&tm_k, (I.j0 + j) * kTileN, head))) break;
             ok = load(&tm_v, (I.j0 + j) * kTileN, head);
           }
+          if (!ok) break;
         }
         // Never leave the CTA with a tensor copy still landing in shared memory.
         if (armed_q) mbar_wait_drain(BAR(kBarQ), (armed_q - 1) & 1);
@@ -231,8 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto k_full = [&](uint32_t g) {
         return mbar_wait_warp(BAR(kBarKFull + g % kStages), (g / kStages) & 1u, abort_flag, p.status);
       };
-      for (int w = w0; ok && w < p.n_items; w += wstep) {
-        const Item I = kv8_item(p, w);
+      while (true) {
+        const Item I = next_item(false, ok);
+        if (!ok || I.w < 0) break;
         const int nA = I.nA, nB = I.nB, n_kv = I.n;
         if (n_kv == 0) continue;
         if (!(ok = mbar_wait_warp(BAR(kBarQ), it & 1u, abort_flag, p.status))) break;
@@ -299,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j1 == n_kv - 1) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
           }
         }
+        if (!ok) break;
         tA += nA;
         tB += nB;
       }
@@ -306,6 +348,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_commit_warp(BAR(kBarDone));
       mbar_wait_drain(BAR(kBarDone), 0);
       __syncwarp();
+    } else if (warp == 14) {
+      // --------------------------------------------------------- scheduler --
+      if (lane == 0) {
+        uint32_t i = 0;
+        for (int w = w0;; w += wstep, ++i) {
+          const bool last = w >= p.n_items;
+          Item I;
+          if (!last)
+            I = kv8_item(p, w);
+          else
+            I.q0 = I.h = I.b = I.kvh = I.len = I.j0 = I.nA = I.nB = I.n = 0, I.w = -1;
+          const uint32_t e = i % kItems;
+          if (!mbar_wait(BAR(kBarItemEmpty + e), ((i / kItems) & 1u) ^ 1u, abort_flag, p.status)) break;
+          const uint32_t at = base + L::kBar + kSlotItem + e * sizeof(Item);
+          st_shared_v4(at, I.q0, I.h, I.b, I.kvh);
+          st_shared_v4(at + 16, I.len, I.j0, I.nA, I.nB);
+          st_shared_v4(at + 32, I.n, I.w, 0, 0);
+          mbar_arrive(BAR(kBarItemFull + e));
+          if (last) break;
+        }
+      }
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AX_KV8_CONVERT_REGS));
@@ -325,8 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       nk = live ? __ldg(p.k_scale + at) : 0.f;
       nv = live ? __ldg(p.v_scale + at) : 0.f;
     };
-    for (int w = w0; ok && w < p.n_items; w += wstep) {
-      const Item I = kv8_item(p, w);
+    while (true) {
+      const Item I = next_item(false, ok);
+      if (!ok || I.w < 0) break;
       if (t < 2 && I.n > 0) scales(I, 0);
       for (int jj = 0; ok && jj < 2 * I.n; ++jj, ++g) {
         const uint32_t slot = g % kRaw, st = (g >> 1) % kStages, use = (g >> 1) / kStages;
@@ -375,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR((is_v ? kBarVFull : kBarKFull) + st));
       }
+      if (!ok) break;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AX_KV8_SOFTMAX_REGS));
@@ -388,8 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t tX = 0;  // tiles of this query tile processed in earlier items
     uint32_t gt = 0;  // key tiles of earlier items
     uint32_t eX = 0;  // epilogues done in earlier items
-    for (int w = w0; ok && w < p.n_items; w += wstep) {
-      const Item I = kv8_item(p, w);
+    while (true) {
+      const Item I = next_item(false, ok);
+      if (!ok || I.w < 0) break;
       const int row = I.q0 + X * kTileM + t;
       const int nX = X ? I.nB : I.nA;
       const int tok = row / p.pack;
@@ -401,20 +467,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[4][32];
-        tmem_ld32(s_addr + 0, s[0]);
-        tmem_ld32(s_addr + 32, s[1]);
-        tmem_ld32(s_addr + 64, s[2]);
-        tmem_ld32(s_addr + 96, s[3]);
-        tmem_ld_wait(s[0]);
-        asm volatile("" : AX_RW32(s[1])::"memory");
-        asm volatile("" : AX_RW32(s[2])::"memory");
-        asm volatile("" : AX_RW32(s[3])::"memory");
-        if (key0 + kTileN > lim) {
+        // The scores are read twice, for the maximum and for the exponentials,
+        // so that they need not stay in registers between the two.
+        const bool edge = key0 + kTileN > lim;
+        uint32_t s[2][32];
+        auto load_block = [&](int i) {  // the scores of 64-key block i, masked
+          tmem_ld32(s_addr + 64 * i, s[0]);
+          tmem_ld32(s_addr + 64 * i + 32, s[1]);
+          tmem_ld_wait(s[0]);
+          asm volatile("" : AX_RW32(s[1])::"memory");
+          if (edge) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (key0 + c >= lim) s[c >> 5][c & 31] = __float_as_uint(-INFINITY);
-        }
+            for (int c = 0; c < 64; ++c)
+              if (key0 + 64 * i + c >= lim) s[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+          }
+        };
         float4 fac[2];  // factor, log2 scale_v, 1 / scale_v of the two blocks
 #pragma unroll
         for (int i = 0; i < 2; ++i) fac[i] = ld_shared_v4f(base + L::kBar + kSlotScale + ((gt + j) & 3) * 32 + i * 16);
@@ -423,13 +490,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         float top[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          load_block(i);
           float mx[4];
 #pragma unroll
           for (int a = 0; a < 4; ++a) {
-            mx[a] = fmax3(SV(64 * i + a), SV(64 * i + a + 4), SV(64 * i + a + 8));
+            mx[a] = fmax3(SV(a), SV(a + 4), SV(a + 8));
 #pragma unroll
-            for (int c = 12; c < 60; c += 8) mx[a] = fmax3(mx[a], SV(64 * i + a + c), SV(64 * i + a + c + 4));
-            mx[a] = fmaxf(mx[a], SV(64 * i + a + 60));
+            for (int c = 12; c < 60; c += 8) mx[a] = fmax3(mx[a], SV(a + c), SV(a + c + 4));
+            mx[a] = fmaxf(mx[a], SV(a + 60));
           }
           top[i] = fmaf(fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]), fac[i].x, fac[i].y);
         }
@@ -455,34 +523,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float base_m = (m == -INFINITY) ? 0.f : m;
-        uint32_t pk[2][32];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
+          load_block(half);
           const float2 mulv = make_float2(fac[half].x, fac[half].x);
           const float off = fac[half].y - base_m;
           const float2 offv = make_float2(off, off);
           float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[32];
 #pragma unroll
-          for (int c = half * 64; c < half * 64 + 64; c += 2) {
+          for (int c = 0; c < 64; c += 2) {
             const float2 x = fma2(make_float2(__uint_as_float(s[c >> 5][c & 31]),
                                               __uint_as_float(s[c >> 5][(c + 1) & 31])),
                                   mulv, offv);
-            float2 pr;
-            if (((c >> 1) & 7) < kPolyPairsPer8) {
-              pr = ex2_poly2(x);
-            } else {
-              pr.x = ex2_approx(x.x);
-              pr.y = ex2_approx(x.y);
-            }
+            const float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
             acc[(c >> 1) & 1] = add2(acc[(c >> 1) & 1], pr);
-            pk[half][(c >> 1) & 31] = pack_half2(pr.x, pr.y);
+            pk[c >> 1] = pack_half2(pr.x, pr.y);
           }
           // Publish this half of P: the MMA warp starts its half of PV_X(j)
           // while the second half is still being computed.
-          tmem_st32(s_addr + half * 32, pk[half]);
+          tmem_st32(s_addr + half * 32, pk);
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(BAR(kBarPHalf + 2 * X + half));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(kBarPHalf + 2 * X + half));
           const float2 a = add2(acc[0], acc[1]);
           l = fmaf(a.x + a.y, fac[half].z, l);
         }
@@ -497,12 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tX += nX;
       gt += I.n;
-      // A row without a visible key has m = -inf and l of masked entries only
-      // (2^-126 each); one with NaN scores has l = NaN.
+      // A row without a visible key has m = -inf and l = 0; one with NaN scores has l = NaN.
       const bool none = nX == 0 || (m == -INFINITY && l == l);
       if (p.n_split > 1) {
         // [item][tile][HD / 4][128 rows] float4, then m and l of the rows.
-        float* part = p.part + (2LL * w + X) * (kTileM * (HD + 2));
+        float* part = p.part + (2LL * I.w + X) * (kTileM * (HD + 2));
         const bool live = row < p.rows;
         if (live) {
           part[kTileM * HD + t] = none ? -INFINITY : m;
