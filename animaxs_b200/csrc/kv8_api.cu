@@ -322,9 +322,8 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   const bool few = p.rows <= 16;
   CUtensorMap tq, tk, tv;
   const int64_t heads = static_cast<int64_t>(cache->batch) * cache->kv_heads;
-  const int box = few ? ax::kKv8Block : ax::kTileN;
-  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, box);
-  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, box);
+  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, ax::kKv8Block);
+  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, ax::kKv8Block);
   if (rc != ANIMAXS_OK) return rc;
   cudaError_t e;
   if (few) {
