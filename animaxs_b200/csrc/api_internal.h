@@ -59,10 +59,10 @@ int ax_make_tmap(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int6
 // swizzled by the row length (64 or 128 bytes).
 int ax_make_tmap_codes(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,
                        int64_t heads, int box_rows);
-// fp16 q as [batch][lines][tokens][pack][dim]; box = 64 columns x pack heads x
-// 128 / pack tokens (128 rows), 128B swizzle.
+// fp16 q or o as [batch][lines][tokens][pack][dim], pack a power of two <= 128;
+// box = 64 columns x box_rows rows (of up to box_rows heads), 128B swizzle.
 int ax_make_tmap_rows(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t pack,
-                      int64_t tokens, int64_t lines, int64_t batch, int64_t st, int64_t sh, int64_t sb);
+                      int64_t tokens, int64_t lines, int64_t batch, int64_t st, int64_t sh, int64_t sb, int box_rows);
 // Peers of a fused head-sharded call: the epilogue stores every output tile
 // also at o + delta[i] and the CTAs count their items on arrive[i].
 struct AxPeers {

@@ -317,7 +317,7 @@ int ax_make_tmap_codes(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base
 }
 
 int ax_make_tmap_rows(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t pack,
-                      int64_t tokens, int64_t lines, int64_t batch, int64_t st, int64_t sh, int64_t sb) {
+                      int64_t tokens, int64_t lines, int64_t batch, int64_t st, int64_t sh, int64_t sb, int box_rows) {
   auto fn = encode_fn();
   if (fn == nullptr)
     return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
@@ -331,7 +331,8 @@ int ax_make_tmap_rows(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base,
                            static_cast<cuuint64_t>(tokens > 1 ? st * 2 : any),
                            static_cast<cuuint64_t>(lines > 1 ? sh * pack * 2 : any),
                            static_cast<cuuint64_t>(batch > 1 ? sb * 2 : any)};
-  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(pack), static_cast<cuuint32_t>(128 / pack), 1, 1};
+  const int64_t heads = pack < box_rows ? pack : box_rows;
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(box_rows / heads), 1, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

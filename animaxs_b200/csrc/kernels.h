@@ -201,11 +201,11 @@ cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const 
                             int dev, cudaStream_t stream);
 
 // Attention over the cache in pairs of 128-row query tiles (kv8_attn_sm100.cu);
-// tq is the 5-D map of ax_make_tmap_rows.
+// tq and to are ax_make_tmap_rows maps of 128 and 32 rows.
 bool kv8_attn_plan(Kv8AttnParams* p, int sms);  // false: too many items
 size_t kv8_attn_part_floats(const Kv8AttnParams& p);
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream);
+                            const CUtensorMap& to, const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream);
 
 // W8 (bits 8) / W4 (bits 4) codes + fp16 scale/zero per row and 64 columns ->
 // fp16 [rows][out_stride] (dequant_sm100.cu).

@@ -320,7 +320,7 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   // Up to 16 rows of a kv head fit the row kernel's one tile, which streams the
   // cache once; more rows are bound by the products and go to the tensor cores.
   const bool few = p.rows <= 16;
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   const int64_t heads = static_cast<int64_t>(cache->batch) * cache->kv_heads;
   rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, ax::kKv8Block);
   if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, ax::kKv8Block);
@@ -340,9 +340,12 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
     rc = ensure_split(ctx, ax::kv8_attn_part_floats(p), 0);
     if (rc != ANIMAXS_OK) return rc;
     p.part = ctx->kv8_part;
-    rc = ax_make_tmap_rows(ctx, &tq, p.q, D, p.pack, p.q_len, p.lines, p.batch, p.q_tok, p.q_head, p.q_batch);
+    rc = ax_make_tmap_rows(ctx, &tq, p.q, D, p.pack, p.q_len, p.lines, p.batch, p.q_tok, p.q_head, p.q_batch,
+                           ax::kTileM);
+    if (rc == ANIMAXS_OK)
+      rc = ax_make_tmap_rows(ctx, &to, p.o, D, p.pack, p.q_len, p.lines, p.batch, p.o_tok, p.o_head, p.o_batch, 32);
     if (rc != ANIMAXS_OK) return rc;
-    e = ax::launch_kv8_attn(tq, tk, tv, p, ctx->num_sms, ctx->device, s);
+    e = ax::launch_kv8_attn(tq, tk, tv, to, p, ctx->num_sms, ctx->device, s);
   }
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "attention launch");
   ctx->last_error.clear();

@@ -18,7 +18,7 @@
 //   0-3, 4-7   softmax of tile A / B: thread t owns row t (= TMEM lane t)
 //   8-11       conversion of each K and V block
 //   12         MMA issuer and TMEM owner
-//   13         TMA producer: Q tiles; code blocks K_0, V_0, K_1, V_1, ... into a 2-slot ring
+//   13         TMA producer: Q tiles; code blocks K_0, V_0, K_1, V_1, ... into a 4-slot ring
 //   14         scheduler: works out the CTA's next items ahead of the other roles
 //              (divisions and the length's load, 2000 cycles when every role did it)
 //   15         idle (it completes the warpgroup)
@@ -42,9 +42,9 @@ namespace ax {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kRaw = 2;     // code slots
+constexpr int kRaw = 4;     // code slots
 constexpr uint32_t kBarBytes = 768;
-constexpr int kStages = 4;  // fp16 K blocks, and V blocks
+constexpr int kStages = 3;  // fp16 K blocks, and V blocks
 constexpr int kBlk = kKv8Block;
 constexpr int kItems = 2;  // items worked out ahead
 constexpr int kItemReaders = 14;
@@ -57,9 +57,9 @@ struct Smem {
   static constexpr uint32_t kK = kQ + 2 * kTile;
   static constexpr uint32_t kV = kK + kStages * kKv;
   static constexpr uint32_t kRing = kV + kStages * kKv;
-  // Output stage: per softmax warp, 32 rows x 32 columns fp16.
+  // Output stage: per softmax warp, 32 rows x 64 columns fp16.
   static constexpr uint32_t kStage = kRing + kRaw * kCodes;
-  static constexpr uint32_t kBar = kStage + 8 * 2048;
+  static constexpr uint32_t kBar = kStage + 8 * 4096;
   static constexpr uint32_t kBytes = kBar + kBarBytes + 1024;  // + alignment slack
 };
 static_assert(Smem<128>::kBytes <= 227 * 1024, "shared memory exceeds the 227 KiB opt-in");
@@ -84,8 +84,8 @@ enum : int {
 constexpr uint32_t kSlotTmem = kNumBars * 8;
 constexpr uint32_t kSlotAbort = kSlotTmem + 4;
 // Per key block: factor of the scores, log2 scale_v, 1 / scale_v (float4, eight
-// blocks deep: K block g is converted after QK(g - 4) retired, which follows
-// the softmax's use of block g - 6).
+// blocks deep: K block g is converted after QK(g - 3) retired, which follows
+// the softmax's use of block g - 5).
 constexpr int kScales = 8;
 constexpr uint32_t kSlotScale = 320;
 constexpr uint32_t kSlotItem = kSlotScale + kScales * 16;  // Item [kItems]
@@ -96,9 +96,9 @@ constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zer
 
 // Register split (setmaxnreg) of the 512 x 128 registers of the launch: softmax
 // 2 x 128 threads, conversion 128, MMA / TMA 128 (build.py checks the sum).
-#define AX_KV8_SOFTMAX_REGS 160
-#define AX_KV8_CONVERT_REGS 96
-#define AX_KV8_OTHER_REGS 96
+#define AX_KV8_SOFTMAX_REGS 176
+#define AX_KV8_CONVERT_REGS 80
+#define AX_KV8_OTHER_REGS 80
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
@@ -143,6 +143,24 @@ __device__ __forceinline__ void issue_pv64(uint32_t d_tmem, uint32_t p_tmem, uin
                      accumulate || kk > 0 ? 1u : 0u);
 }
 
+// Place in a ring of kStages: stage, and parity of the phase its use completes.
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+__device__ __forceinline__ void tma_store_5d(const void* tmap, uint32_t src, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];" ::"l"(tmap),
+      "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
 struct alignas(16) Item {
   int q0, h, b, kvh;
   int len;
@@ -185,7 +203,8 @@ __device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_attn_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                          const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
+                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                          const Kv8AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -222,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_o);
   }
   tc_fence_before();
   __syncthreads();
@@ -300,18 +320,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 12) {
       // --------------------------------------------------------------- MMA --
-      uint32_t gk = 0, gv = 0;  // K / V blocks consumed so far
+      Ring gk, gv;              // the next K / V block
       uint32_t tA = 0, tB = 0;  // blocks of A / B in earlier items
       bool ok = true;
       uint32_t it = 0;
       auto k_full = [&] {
-        const bool r = mbar_wait_warp(BAR(kBarKFull + gk % kStages), (gk / kStages) & 1u, abort_flag, p.status);
+        const bool r = mbar_wait_warp(BAR(kBarKFull + gk.stage), gk.phase, abort_flag, p.status);
         tc_fence_after();
         return r;
       };
       // QK of tile X's block number t (a running count) with K block gk, into buffer t % 2.
       auto qk = [&](int X, uint32_t t) {
-        issue_qk64<HD>(tmem + X * 128 + (t & 1u) * 64, sQ + X * L::kTile, sK + (gk % kStages) * L::kKv);
+        issue_qk64<HD>(tmem + X * 128 + (t & 1u) * 64, sQ + X * L::kTile, sK + (gk.stage) * L::kKv);
         tc_commit_warp(BAR(kBarSFull + 2 * X + (t & 1u)));
       };
       // PV of block t once its P is published.  An item's first P is published
@@ -319,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto pv = [&](int X, uint32_t t, bool accumulate) -> bool {
         if (!mbar_wait_warp(BAR(kBarPFull + 2 * X + (t & 1u)), (t >> 1) & 1u, abort_flag, p.status)) return false;
         tc_fence_after();
-        issue_pv64<HD>(tmem + kColO + X * HD, tmem + X * 128 + (t & 1u) * 64, sV + (gv % kStages) * L::kKv, accumulate);
+        issue_pv64<HD>(tmem + kColO + X * HD, tmem + X * 128 + (t & 1u) * 64, sV + (gv.stage) * L::kKv, accumulate);
         return true;
       };
       while (true) {
@@ -333,14 +353,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = k_full())) break;
           if (j < nA) qk(0, tA + j);
           if (j < nB) qk(1, tB + j);
-          tc_commit_warp(BAR(kBarKEmpty + gk % kStages));
-          ++gk;
+          tc_commit_warp(BAR(kBarKEmpty + gk.stage));
+          gk.next();
         }
         if (!ok) break;
         if (n <= 2) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
         // A buffer's next scores follow the PV that reads its P (same thread, issue order).
         for (int j = 0; j < n; ++j) {
-          if (!(ok = mbar_wait_warp(BAR(kBarVFull + gv % kStages), (gv / kStages) & 1u, abort_flag, p.status))) break;
+          if (!(ok = mbar_wait_warp(BAR(kBarVFull + gv.stage), gv.phase, abort_flag, p.status))) break;
           if (j < nA) {
             if (!(ok = pv(0, tA + j, j > 0))) break;
             if (j == nA - 1) tc_commit_warp(BAR(kBarODone + 0));
@@ -351,12 +371,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = pv(1, tB + j, j > 0))) break;
             if (j == nB - 1) tc_commit_warp(BAR(kBarODone + 1));
           }
-          tc_commit_warp(BAR(kBarVEmpty + gv % kStages));
-          ++gv;
+          tc_commit_warp(BAR(kBarVEmpty + gv.stage));
+          gv.next();
           if (j + 2 < nB) qk(1, tB + j + 2);
           if (j + 2 < n) {
-            tc_commit_warp(BAR(kBarKEmpty + gk % kStages));
-            ++gk;
+            tc_commit_warp(BAR(kBarKEmpty + gk.stage));
+            gk.next();
             if (j + 2 == n - 1) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
           }
         }
@@ -400,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x - 256;
     const int key = t & 63, part = t >> 6;
     uint32_t g = 0;  // code blocks taken so far: K and V alternate
+    Ring r;
     bool ok = true;
     float nk = 0.f, nv = 0.f;  // thread 0: scales of the next K block
     auto scales = [&](const Item& I, int j) {
@@ -412,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok || I.w < 0) break;
       if (t == 0 && I.n > 0) scales(I, 0);
       for (int jj = 0; ok && jj < 2 * I.n; ++jj, ++g) {
-        const uint32_t st = (g >> 1) % kStages, use = (g >> 1) / kStages;
         const bool is_v = (g & 1u) != 0;
         const uint32_t slot = g % kRaw;
         ok = mbar_wait_warp(BAR(kBarRawFull + slot), (g / kRaw) & 1u, abort_flag, p.status);
@@ -431,9 +451,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-        ok = mbar_wait_warp(BAR((is_v ? kBarVEmpty : kBarKEmpty) + st), (use & 1u) ^ 1u, abort_flag, p.status);
+        ok = mbar_wait_warp(BAR((is_v ? kBarVEmpty : kBarKEmpty) + r.stage), r.phase ^ 1u, abort_flag, p.status);
         if (!ok) break;
-        const uint32_t dst = (is_v ? sV : sK) + st * L::kKv + key * 128;
+        const uint32_t dst = (is_v ? sV : sK) + r.stage * L::kKv + key * 128;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
           uint32_t h[8];
@@ -458,7 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(BAR((is_v ? kBarVFull : kBarKFull) + st));
+        if (lane == 0) mbar_arrive(BAR((is_v ? kBarVFull : kBarKFull) + r.stage));
+        if (is_v) r.next();  // K and V blocks alternate: both rings stand at the same place
       }
       if (!ok) break;
     }
@@ -594,46 +615,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        // Each warp stages its 32 rows, 32 columns at a time (16-byte unit u of
-        // row r at unit u ^ (r / 2 % 4)), and stores 64 contiguous bytes a row
-        // with four lanes; a thread storing its own row took 5500 cycles an item.
+        // Each warp stages its 32 rows, 64 columns at a time, in the tensor-store
+        // layout (16-byte unit u of row r at unit u ^ (r % 8)) and its lane 0
+        // writes them with one TMA store; rows past the last are clipped.  (Plain
+        // stores, even four lanes to a row, kept the load/store unit busy for
+        // 2000 cycles an item.)
         const float inv_l = none ? 0.f : 1.f / l;
-        const uint32_t stage = base + L::kStage + static_cast<uint32_t>(warp) * 2048u;
-        const int line = I.q0 + X * kTileM + (warp & 3) * 32 + (lane >> 2);  // the lane's first row to store
-        __half* dst[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = line + 8 * i;
-          const int head = I.h * p.pack + (r & (p.pack - 1));
-          dst[i] = p.o + I.b * p.o_batch + static_cast<long long>(r >> p.pack_log2) * p.o_tok + head * p.o_head +
-                   (lane & 3) * 8;
-        }
+        const uint32_t wstage = base + L::kStage + static_cast<uint32_t>(warp) * 4096u;
+        const uint32_t stage = wstage + lane * 128u;
+        const int row0 = I.q0 + X * kTileM + (warp & 3) * 32;
 #pragma unroll 1
-        for (int c4 = 0; c4 < HD / 32; ++c4) {
-          uint32_t o[32];
-          if (nX > 0) {
-            tmem_ld32(o_addr + c4 * 32, o);
-            tmem_ld_wait(o);
-          }
-          __syncwarp();  // the stage's last round has been read
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint32_t* v = &o[u * 8];
-            const uint32_t at = stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4);
-            if (none)
-              st_shared_v4(at, 0u, 0u, 0u, 0u);
-            else
-              st_shared_v4(at, pack_half2(__uint_as_float(v[0]) * inv_l, __uint_as_float(v[1]) * inv_l),
-                           pack_half2(__uint_as_float(v[2]) * inv_l, __uint_as_float(v[3]) * inv_l),
-                           pack_half2(__uint_as_float(v[4]) * inv_l, __uint_as_float(v[5]) * inv_l),
-                           pack_half2(__uint_as_float(v[6]) * inv_l, __uint_as_float(v[7]) * inv_l));
-          }
+        for (int rd = 0; rd < HD / 64; ++rd) {
+          uint32_t o[2][32];
+          tmem_ld32(o_addr + rd * 64, o[0]);  // stale where the item has no keys: replaced by zeros below
+          tmem_ld32(o_addr + rd * 64 + 32, o[1]);
+          tmem_ld_wait(o[0]);
+          asm volatile("" : AX_RW32(o[1])::"memory");
+          // The stage's previous store (last round or item) has been read.
+          if (lane == 0) tma_store_wait_read();
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2);
-            const uint4 v = ld_shared_v4u(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-            if (line + 8 * i < p.rows) *reinterpret_cast<uint4*>(dst[i] + c4 * 32) = v;
+          for (int u = 0; u < 8; ++u) {
+            const uint32_t* v = &o[u >> 2][(u & 3) * 8];
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              h[i] = pack_half2(__uint_as_float(v[2 * i]) * inv_l, __uint_as_float(v[2 * i + 1]) * inv_l);
+              if (none) h[i] = 0u;
+            }
+            st_shared_v4(stage + ((u ^ (lane & 7)) << 4), h[0], h[1], h[2], h[3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.rows) {
+            tma_store_5d(&tm_o, wstage, 64 * rd, row0 & (p.pack - 1), row0 >> p.pack_log2, I.h, I.b);
+            tma_store_commit();
           }
         }
       }
@@ -641,6 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (warp < 8 && lane == 0) tma_store_wait_all();  // the output stores have completed
   tc_fence_before();
   __syncthreads();
   if (warp == 12) {
@@ -690,8 +707,8 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
 }
 
 template <int FMT, int HD>
-cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p,
-                      int grid, int dev, cudaStream_t stream) {
+cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
+                      const Kv8AttnParams& p, int grid, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
   const uint64_t bit = 1ull << (dev & 63);
   auto kernel = kv8_attn_sm100_kernel<FMT, HD>;
@@ -700,7 +717,7 @@ cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
-  kernel<<<grid, kThreads, Smem<HD>::kBytes, stream>>>(tq, tk, tv, p);
+  kernel<<<grid, kThreads, Smem<HD>::kBytes, stream>>>(tq, tk, tv, to, p);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && p.n_split > 1) {
     const int blocks = p.batch * p.lines * p.pairs * 2 * (HD / 8);
@@ -745,13 +762,13 @@ size_t kv8_attn_part_floats(const Kv8AttnParams& p) {
 }
 
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream) {
+                            const CUtensorMap& to, const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream) {
   const int grid = p.n_items < sms ? p.n_items : sms;
   if (p.format == kKv8Int8)
-    return p.head_dim == 128 ? launch_hd<kKv8Int8, 128>(tq, tk, tv, p, grid, dev, stream)
-                             : launch_hd<kKv8Int8, 64>(tq, tk, tv, p, grid, dev, stream);
-  return p.head_dim == 128 ? launch_hd<kKv8E4m3, 128>(tq, tk, tv, p, grid, dev, stream)
-                           : launch_hd<kKv8E4m3, 64>(tq, tk, tv, p, grid, dev, stream);
+    return p.head_dim == 128 ? launch_hd<kKv8Int8, 128>(tq, tk, tv, to, p, grid, dev, stream)
+                             : launch_hd<kKv8Int8, 64>(tq, tk, tv, to, p, grid, dev, stream);
+  return p.head_dim == 128 ? launch_hd<kKv8E4m3, 128>(tq, tk, tv, to, p, grid, dev, stream)
+                           : launch_hd<kKv8E4m3, 64>(tq, tk, tv, to, p, grid, dev, stream);
 }
 
 }  // namespace ax
