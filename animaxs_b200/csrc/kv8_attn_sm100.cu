@@ -17,11 +17,11 @@
 // round-robin to one persistent CTA per SM.  Sixteen warps:
 //   0-3, 4-7   softmax of tile A / B: thread t owns row t (= TMEM lane t)
 //   8-11       conversion of each K and V block
-//   12         MMA issuer and TMEM owner
-//   13         TMA producer: Q tiles; code blocks K_0, V_0, K_1, V_1, ... into a 4-slot ring
+//   12, 15     MMA issuers of tile A / B (12 owns TMEM); one warp for both spent
+//              2300 cycles a block on its waits, commits and issues
+//   13         TMA producer: Q tiles; code blocks K_0, V_0, K_1, V_1, ... into a 2-slot ring
 //   14         scheduler: works out the CTA's next items ahead of the other roles
 //              (divisions and the length's load, 2000 cycles when every role did it)
-//   15         idle (it completes the warpgroup)
 // TMEM (512 columns): scores of tile A in two buffers of 64 columns, [0,64) and
 // [64,128), of tile B in [128,192) and [192,256), O_A [256,..), O_B.  P (fp16)
 // overlays the first half of the scores it came from.  With two buffers the
@@ -42,12 +42,12 @@ namespace ax {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kRaw = 4;     // code slots
+constexpr int kRaw = 2;     // code slots
 constexpr uint32_t kBarBytes = 768;
-constexpr int kStages = 3;  // fp16 K blocks, and V blocks
+constexpr int kKStages = 4, kVStages = 3;  // fp16 blocks
 constexpr int kBlk = kKv8Block;
 constexpr int kItems = 2;  // items worked out ahead
-constexpr int kItemReaders = 14;
+constexpr int kItemReaders = 15;
 template <int HD>
 struct Smem {
   static constexpr uint32_t kTile = kTileM * HD * 2;  // fp16 query tile
@@ -55,8 +55,8 @@ struct Smem {
   static constexpr uint32_t kCodes = kBlk * HD;       // its codes
   static constexpr uint32_t kQ = 0;                      // Q_A, Q_B
   static constexpr uint32_t kK = kQ + 2 * kTile;
-  static constexpr uint32_t kV = kK + kStages * kKv;
-  static constexpr uint32_t kRing = kV + kStages * kKv;
+  static constexpr uint32_t kV = kK + kKStages * kKv;
+  static constexpr uint32_t kRing = kV + kVStages * kKv;
   // Output stage: per softmax warp, 32 rows x 64 columns fp16.
   static constexpr uint32_t kStage = kRing + kRaw * kCodes;
   static constexpr uint32_t kBar = kStage + 8 * 4096;
@@ -69,23 +69,22 @@ enum : int {
   kBarRawFull,                             // +slot
   kBarRawEmpty = kBarRawFull + kRaw,       // +slot (4 warp arrivals)
   kBarKFull = kBarRawEmpty + kRaw,         // +stage (4 warp arrivals)
-  kBarKEmpty = kBarKFull + kStages,        // +stage
-  kBarVFull = kBarKEmpty + kStages,        // +stage (4 warp arrivals)
-  kBarVEmpty = kBarVFull + kStages,        // +stage
-  kBarSFull = kBarVEmpty + kStages,        // +2*tile + buffer
+  kBarVFull = kBarKFull + kKStages,        // +stage (4 warp arrivals)
+  kBarVEmpty = kBarVFull + kVStages,       // +stage (2: tile A, tile B): the block's PVs have retired
+  kBarSFull = kBarVEmpty + kVStages,       // +2*tile + buffer
   kBarPFull = kBarSFull + 4,               // +2*tile + buffer (4 warp arrivals)
   kBarODone = kBarPFull + 4,               // +tile
-  kBarQFree = kBarODone + 2,
+  kBarQFree = kBarODone + 2,               // (2: tile A, tile B)
   kBarItemFull,                            // +entry
-  kBarItemEmpty = kBarItemFull + kItems,   // +entry (14 arrivals: every consuming warp)
-  kBarDone = kBarItemEmpty + kItems,
-  kNumBars
+  kBarItemEmpty = kBarItemFull + kItems,   // +entry (15 arrivals: every consuming warp)
+  kBarDone = kBarItemEmpty + kItems,       // +tile
+  kNumBars = kBarDone + 2
 };
 constexpr uint32_t kSlotTmem = kNumBars * 8;
 constexpr uint32_t kSlotAbort = kSlotTmem + 4;
 // Per key block: factor of the scores, log2 scale_v, 1 / scale_v (float4, eight
-// blocks deep: K block g is converted after QK(g - 3) retired, which follows
-// the softmax's use of block g - 5).
+// blocks deep: K block g is converted after PV(g - 4) retired, which follows
+// the softmax's use of block g - 4).
 constexpr int kScales = 8;
 constexpr uint32_t kSlotScale = 320;
 constexpr uint32_t kSlotItem = kSlotScale + kScales * 16;  // Item [kItems]
@@ -143,11 +142,12 @@ __device__ __forceinline__ void issue_pv64(uint32_t d_tmem, uint32_t p_tmem, uin
                      accumulate || kk > 0 ? 1u : 0u);
 }
 
-// Place in a ring of kStages: stage, and parity of the phase its use completes.
+// Place in a ring: stage, and parity of the phase its use completes.
+template <int N>
 struct Ring {
   uint32_t stage = 0, phase = 0;
   __device__ __forceinline__ void next() {
-    if (++stage == kStages) {
+    if (++stage == N) {
       stage = 0;
       phase ^= 1u;
     }
@@ -224,8 +224,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kNumBars; ++i) {
       uint32_t count = 1;
       if (i >= kBarRawEmpty && i < kBarRawEmpty + kRaw) count = 4;
-      if (i >= kBarKFull && i < kBarKFull + kStages) count = 4;
-      if (i >= kBarVFull && i < kBarVFull + kStages) count = 4;
+      if (i >= kBarKFull && i < kBarKFull + kKStages) count = 4;
+      if (i >= kBarVFull && i < kBarVFull + kVStages) count = 4;
+      if (i >= kBarVEmpty && i < kBarVEmpty + kVStages) count = 2;
+      if (i == kBarQFree) count = 2;
       if (i >= kBarPFull && i < kBarPFull + 4) count = 4;
       if (i >= kBarItemEmpty && i < kBarItemEmpty + kItems) count = kItemReaders;
       mbar_init(BAR(i), count);
@@ -318,75 +320,70 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kRaw; ++s)
           if (armed[s]) mbar_wait_drain(BAR(kBarRawFull + s), (armed[s] - 1) & 1);
       }
-    } else if (warp == 12) {
+    } else if (warp == 12 || warp == 15) {
       // --------------------------------------------------------------- MMA --
-      Ring gk, gv;              // the next K / V block
-      uint32_t tA = 0, tB = 0;  // blocks of A / B in earlier items
+      // One warp per query tile; both count every block of an item in and out,
+      // so that a stage is free when both are past it.
+      const int X = warp == 12 ? 0 : 1;
+      const uint32_t tS = tmem + X * 128, tO = tmem + kColO + X * HD, q_tile = sQ + X * L::kTile;
+      Ring<kKStages> gk;  // the next K block
+      Ring<kVStages> gv;  // the next V block
+      uint32_t tX = 0;    // blocks of this tile in earlier items
       bool ok = true;
       uint32_t it = 0;
-      auto k_full = [&] {
-        const bool r = mbar_wait_warp(BAR(kBarKFull + gk.stage), gk.phase, abort_flag, p.status);
+      // QK of the tile's block number t (a running count) into score buffer t % 2.
+      auto qk = [&](uint32_t t) -> bool {
+        if (!mbar_wait_warp(BAR(kBarKFull + gk.stage), gk.phase, abort_flag, p.status)) return false;
         tc_fence_after();
-        return r;
-      };
-      // QK of tile X's block number t (a running count) with K block gk, into buffer t % 2.
-      auto qk = [&](int X, uint32_t t) {
-        issue_qk64<HD>(tmem + X * 128 + (t & 1u) * 64, sQ + X * L::kTile, sK + (gk.stage) * L::kKv);
+        issue_qk64<HD>(tS + (t & 1u) * 64, q_tile, sK + gk.stage * L::kKv);
         tc_commit_warp(BAR(kBarSFull + 2 * X + (t & 1u)));
-      };
-      // PV of block t once its P is published.  An item's first P is published
-      // after the previous epilogue has read O out of TMEM.
-      auto pv = [&](int X, uint32_t t, bool accumulate) -> bool {
-        if (!mbar_wait_warp(BAR(kBarPFull + 2 * X + (t & 1u)), (t >> 1) & 1u, abort_flag, p.status)) return false;
-        tc_fence_after();
-        issue_pv64<HD>(tmem + kColO + X * HD, tmem + X * 128 + (t & 1u) * 64, sV + (gv.stage) * L::kKv, accumulate);
+        gk.next();
         return true;
       };
       while (true) {
         const Item I = next_item(false, ok);
         if (!ok || I.w < 0) break;
-        const int nA = I.nA, nB = I.nB, n = I.n;
+        const int n = I.n, nX = X ? I.nB : I.nA;
         if (n == 0) continue;
         if (!(ok = mbar_wait_warp(BAR(kBarQ), it & 1u, abort_flag, p.status))) break;
         ++it;
-        for (int j = 0; j < 2 && j < n; ++j) {
-          if (!(ok = k_full())) break;
-          if (j < nA) qk(0, tA + j);
-          if (j < nB) qk(1, tB + j);
-          tc_commit_warp(BAR(kBarKEmpty + gk.stage));
-          gk.next();
-        }
+        for (int j = 0; ok && j < 2 && j < nX; ++j) ok = qk(tX + j);
         if (!ok) break;
-        if (n <= 2) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
-        // A buffer's next scores follow the PV that reads its P (same thread, issue order).
-        for (int j = 0; j < n; ++j) {
-          if (!(ok = mbar_wait_warp(BAR(kBarVFull + gv.stage), gv.phase, abort_flag, p.status))) break;
-          if (j < nA) {
-            if (!(ok = pv(0, tA + j, j > 0))) break;
-            if (j == nA - 1) tc_commit_warp(BAR(kBarODone + 0));
-          }
-          if (j + 2 < n && !(ok = k_full())) break;
-          if (j + 2 < nA) qk(0, tA + j + 2);
-          if (j < nB) {
-            if (!(ok = pv(1, tB + j, j > 0))) break;
-            if (j == nB - 1) tc_commit_warp(BAR(kBarODone + 1));
-          }
+        if (nX > 0 && nX <= 2) tc_commit_warp(BAR(kBarQFree));  // the tile's last QK
+        for (int j = 0; j < nX; ++j) {
+          // V block j was converted before K block j + 1, which this warp has
+          // waited for already, unless j is the last.
+          if (j == nX - 1 && !(ok = mbar_wait_warp(BAR(kBarVFull + gv.stage), gv.phase, abort_flag, p.status))) break;
+          const uint32_t t = tX + j;
+          // An item's first P is published after the previous epilogue has read O.
+          if (!(ok = mbar_wait_warp(BAR(kBarPFull + 2 * X + (t & 1u)), (t >> 1) & 1u, abort_flag, p.status))) break;
+          tc_fence_after();
+          issue_pv64<HD>(tO, tS + (t & 1u) * 64, sV + gv.stage * L::kKv, j > 0);
+          if (j == nX - 1) tc_commit_warp(BAR(kBarODone + X));
           tc_commit_warp(BAR(kBarVEmpty + gv.stage));
           gv.next();
-          if (j + 2 < nB) qk(1, tB + j + 2);
-          if (j + 2 < n) {
-            tc_commit_warp(BAR(kBarKEmpty + gk.stage));
-            gk.next();
-            if (j + 2 == n - 1) tc_commit_warp(BAR(kBarQFree));  // the item's last QK
+          // A buffer's next scores follow the PV that reads its P (same thread, issue order).
+          if (j + 2 < nX) {
+            if (!(ok = qk(t + 2))) break;
+            if (j + 2 == nX - 1) tc_commit_warp(BAR(kBarQFree));
           }
         }
         if (!ok) break;
-        tA += nA;
-        tB += nB;
+        tX += nX;
+        if (nX == 0 && lane == 0) mbar_arrive(BAR(kBarQFree));
+        // Blocks that only the other tile reads: past them once they are there
+        // (an earlier arrival could count for the stage's previous use).
+        for (int j = nX; j < n; ++j) {
+          if (!(ok = mbar_wait_warp(BAR(kBarVFull + gv.stage), gv.phase, abort_flag, p.status))) break;
+          if (lane == 0) mbar_arrive(BAR(kBarVEmpty + gv.stage));
+          gk.next();
+          gv.next();
+        }
+        if (!ok) break;
       }
       // All MMAs this warp issued must retire before TMEM is released.
-      tc_commit_warp(BAR(kBarDone));
-      mbar_wait_drain(BAR(kBarDone), 0);
+      tc_commit_warp(BAR(kBarDone + X));
+      mbar_wait_drain(BAR(kBarDone + X), 0);
       __syncwarp();
     } else if (warp == 14) {
       // --------------------------------------------------------- scheduler --
@@ -420,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x - 256;
     const int key = t & 63, part = t >> 6;
     uint32_t g = 0;  // code blocks taken so far: K and V alternate
-    Ring r;
+    Ring<kKStages> rk;
+    Ring<kVStages> rv;
     bool ok = true;
     float nk = 0.f, nv = 0.f;  // thread 0: scales of the next K block
     auto scales = [&](const Item& I, int j) {
@@ -451,9 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-        ok = mbar_wait_warp(BAR((is_v ? kBarVEmpty : kBarKEmpty) + r.stage), r.phase ^ 1u, abort_flag, p.status);
+        // K block g takes the stage of K block g - 4, whose QKs retired before the
+        // PVs of block g - 4, which V block g - 1 has waited for.
+        if (is_v) ok = mbar_wait_warp(BAR(kBarVEmpty + rv.stage), rv.phase ^ 1u, abort_flag, p.status);
         if (!ok) break;
-        const uint32_t dst = (is_v ? sV : sK) + r.stage * L::kKv + key * 128;
+        const uint32_t dst = (is_v ? sV + rv.stage * L::kKv : sK + rk.stage * L::kKv) + key * 128;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
           uint32_t h[8];
@@ -478,8 +478,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(BAR((is_v ? kBarVFull : kBarKFull) + r.stage));
-        if (is_v) r.next();  // K and V blocks alternate: both rings stand at the same place
+        if (is_v) {
+          if (lane == 0) mbar_arrive(BAR(kBarVFull + rv.stage));
+          rv.next();
+        } else {
+          if (lane == 0) mbar_arrive(BAR(kBarKFull + rk.stage));
+          rk.next();
+        }
       }
       if (!ok) break;
     }
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // when its PVs have retired, and PV_X(j) starts only after this warp's
           // arrival below, so the phase waited for cannot be passed.
           const uint32_t v = gt + j - 1;
-          ok = mbar_wait(BAR(kBarVEmpty + v % kStages), (v / kStages) & 1u, abort_flag, p.status);
+          ok = mbar_wait(BAR(kBarVEmpty + v % kVStages), (v / kVStages) & 1u, abort_flag, p.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
