@@ -184,24 +184,24 @@ struct Kv8AttnParams {
   const float* k_scale;
   const float* v_scale;
   int rows;             // group * q_len: query rows of a kv head
-  int row_tiles;        // 16-row tiles of them
   float* part;          // workspace: partial results (kv8_rows_part_floats, kv8_attn_part_floats)
-  unsigned int* count;  // arrivals per (sequence, kv head, row tile), zero between launches
+  unsigned int* count;  // arrivals per (sequence, kv head), zero between launches
   unsigned int* status;
   // Many rows (kv8_attn_plan): heads of a row line, row lines per sequence,
   // pairs of query tiles per line, parts of the keys, work items.  `rows` is
   // then the rows of a line.
   int pack, pack_log2, lines, pairs, n_split, n_items;
 };
-// Attention over the cache in tiles of 16 query rows (kv8_rows_sm100.cu).  Here and
-// below tk/tv are ax_make_tmap_codes maps with 64-row boxes.
+// Attention of up to 16 query rows over the cache (kv8_rows_sm100.cu); tk/tv are
+// ax_make_tmap_codes maps with boxes of kv8_rows_tile() rows.
+int kv8_rows_tile();
 int kv8_rows_grid(const Kv8AttnParams& p, int sms);
 size_t kv8_rows_part_floats(int head_dim, int grid);
 cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid,
                             int dev, cudaStream_t stream);
 
 // Attention over the cache in pairs of 128-row query tiles (kv8_attn_sm100.cu);
-// tq and to are ax_make_tmap_rows maps of 128 and 32 rows.
+// tk/tv have 64-row boxes, tq and to are ax_make_tmap_rows maps of 128 and 32 rows.
 bool kv8_attn_plan(Kv8AttnParams* p, int sms);  // false: too many items
 size_t kv8_attn_part_floats(const Kv8AttnParams& p);
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,

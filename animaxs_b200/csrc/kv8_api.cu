@@ -322,12 +322,12 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   const bool few = p.rows <= 16;
   CUtensorMap tq, tk, tv, to;
   const int64_t heads = static_cast<int64_t>(cache->batch) * cache->kv_heads;
-  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, ax::kKv8Block);
-  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, ax::kKv8Block);
+  const int box = few ? ax::kv8_rows_tile() : ax::kKv8Block;
+  rc = ax_make_tmap_codes(ctx, &tk, cache->k_codes, D, cache->capacity, heads, box);
+  if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, box);
   if (rc != ANIMAXS_OK) return rc;
   cudaError_t e;
   if (few) {
-    p.row_tiles = 1;
     const int grid = ax::kv8_rows_grid(p, ctx->num_sms);
     rc = ensure_split(ctx, ax::kv8_rows_part_floats(d->head_dim, grid), static_cast<size_t>(heads));
     if (rc != ANIMAXS_OK) return rc;

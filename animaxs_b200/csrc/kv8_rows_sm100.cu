@@ -1,9 +1,9 @@
 // kv8_rows_sm100.cu -- attention of a few query rows over the 8-bit K/V cache.
 //
-// A kv head's query rows (its query heads x the call's query tokens) are taken
-// 16 at a time, so that each code is read and converted once for all of them.
-// With r rows the kernel does 4 r flops a code byte: at a few rows HBM bounds
-// it, and everything here serves to keep loads in flight.
+// A kv head's query rows (its query heads x the call's query tokens, up to 16)
+// are taken together, so that each code is read and converted once for all of
+// them.  With r rows the kernel does 4 r flops a code byte: HBM bounds it, and
+// everything here serves to keep loads in flight and the conversion cheap.
 //
 // Mathematics, per 64-key block c (the tokens that share a scale): with
 // acc = q . code_k,
@@ -14,23 +14,24 @@
 // anyway, p' never exceeds 2^8 (see the lazy rescale below) whatever the
 // scales, and the codes enter both products unscaled, exact as fp16.
 //
-// Work: every (sequence, kv head, row tile) is a row of key tiles of 64; all
-// of them together form one line of tiles that is cut into equal contiguous
-// shares, one per CTA (two CTAs per SM), so ragged lengths and single long
-// sequences load the SMs alike.  A CTA that covers only part of a sequence's
-// keys stores (m', l, O') in its workspace slot and counts itself in; the last
-// one to arrive joins the parts in CTA order, so the result does not depend on
-// the order of arrival.
+// Work: every (sequence, kv head) is a line of 32-key tiles; all lines together
+// are cut into equal contiguous shares, one per warp (eight warps per SM), so
+// ragged lengths and single long sequences load the SMs alike.  A warp runs by
+// itself: its lane 0 keeps a ring of tiles in flight by TMA, all lanes take a
+// tile into registers, and no other warp is waited for until the share is done.
+// Then the CTA's warps join the parts of lines that cross a warp's share, and
+// what crosses the CTA's goes through a workspace: each CTA stores its part
+// (m', l, O') and counts itself in, and the last one to arrive joins the
+// parts in CTA order, so the result does not depend on the order of arrival.
 //
-// A CTA: warp 4 loads tiles (16 KiB: 64 K rows, 64 V rows) by TMA into a ring;
-// warps 0-3 take 16 keys of each tile each, with their own m', l, O' and no
-// synchronisation among them until the CTA leaves the sequence.  The products
-// are m16n8k16 mma.sync: with at most 16 rows a 128-row tcgen05 tile would be
-// mostly empty, and reading codes from shared memory into fragments and
-// converting them there avoids a second pass through shared memory.  Which of
-// a row's codes form an MMA's k (for K) or n (for V) index is free as long as Q,
-// or the stored O, follows: a lane takes 16-byte runs of a row (32 codes
-// of one K row, 16 of each of its four V rows), which TMA's swizzle spreads over all banks.
+// Products: m16n8k16 mma.sync with the cache as the 16-wide operand and the
+// query rows as the 8-wide one (one or two column tiles):
+//   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 d x 8 rows] += V^T P^T.
+// A 128-row tcgen05 tile would be mostly empty at these row counts, and codes
+// would have to pass through shared memory a second time.  Which codes of a
+// row form an MMA's k index (K) or m index (V) is free as long as Q, or the
+// stored O, follows: a lane takes 16-byte runs (32 codes of each of two K
+// rows, 16 of each of four V rows), which TMA's swizzle spreads over the banks.
 #include <atomic>
 
 #include "api_internal.h"
@@ -41,31 +42,43 @@
 namespace ax {
 namespace {
 
-constexpr int kStages = 4;
-constexpr int kConsumers = 128;
-constexpr int kThreads = kConsumers + 32;
-constexpr int kCtasPerSm = 2;
-constexpr float kRescale = 8.f;  // log2 units by which the maximum may lag
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTileKeys = 32;
+constexpr float kRescale = 8.f;    // log2 units by which the maximum may lag
 constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
-template <int HD>
+// NT: column tiles of 8 query rows (1 or 2).
+template <int HD, int NT>
 struct RowsSmem {
-  static constexpr uint32_t kTile = kKv8Block * HD;             // codes of K (or V) of a tile
-  static constexpr uint32_t kRing = 0;
-  static constexpr uint32_t kMerge = kRing + kStages * 2 * kTile;  // [4 warps][16 rows][HD] fp32
-  static constexpr uint32_t kStat = kMerge + 4 * 16 * HD * 4;      // [4 warps][16 rows] m', l
-  static constexpr uint32_t kPrefix = kStat + 4 * 16 * 8;          // tiles of the sequences before each share
-  static constexpr uint32_t kBar = kPrefix + (kConsumers + 1) * 8 + 8;
-  static constexpr uint32_t kBytes = kBar + 2 * kStages * 8 + 16 + 1024;  // + alignment slack
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kStages = NT == 1 ? 3 : 2;
+  static constexpr uint32_t kCodes = kTileKeys * HD;              // codes of K (or V) of a tile
+  static constexpr uint32_t kRing = kWarps * kStages * 2 * kCodes;
+  static constexpr uint32_t kSlot = kRows * (HD + 2) * 4;         // O' [rows][HD], m' [rows], l [rows]
+  static constexpr uint32_t kHead = kRing;                        // [warp] part of the share's first line
+  static constexpr uint32_t kPrefix = kHead + kWarps * kSlot;     // int32 [kThreads + 1]
+  static constexpr uint32_t kBar = (kPrefix + (kThreads + 1) * 4 + 15) / 16 * 16;
+  static constexpr uint32_t kInfo = kBar + kWarps * kStages * 8;  // int [2 * warp]: line of the slot, -1: none
+  static constexpr uint32_t kBytes = kInfo + 2 * kWarps * 4 + 16 + 1024;  // + alignment slack
+  // The part of a share's last line goes to the warp's own ring, which is idle by then.
+  static_assert(kStages * 2 * kCodes >= kSlot, "a slot must fit a warp's ring");
+  static_assert(kBytes <= 227 * 1024, "shared memory exceeds the 227 KiB opt-in");
 };
-static_assert(2 * (RowsSmem<128>::kBytes + 1024) <= 228 * 1024, "two CTAs must fit on an SM");
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8 x 8 matrix of 16-bit values held one row per four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
 }
 __device__ __forceinline__ uint2 ld_shared_v2u(uint32_t addr) {
   uint2 v;
@@ -80,473 +93,543 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
-// A place in the line of tiles: tile `tile` of `tiles` of (sequence b, row line
-// hr = kv head * row_tiles + row tile).
+// A place among the tiles: tile `tile` of `tiles` of kv head h of sequence b.
 struct Place {
-  int b, hr, tile, tiles;
+  int b, h, tile, tiles;
 };
 
-template <int FMT, int HD>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+template <int FMT, int HD, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
     kv8_rows_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                           const Kv8AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
-  using L = RowsSmem<HD>;
+  using L = RowsSmem<HD, NT>;
+  constexpr int kStages = L::kStages;
+  constexpr int kF4 = HD / 4;  // float4 units of a row
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  float* stat = reinterpret_cast<float*>(gbase + L::kStat);
-  long long* prefix = reinterpret_cast<long long*>(gbase + L::kPrefix);
-  const uint32_t bar_full = base + L::kBar, bar_empty = bar_full + 8 * kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kBar + 16 * kStages);
-  volatile unsigned* last_flag = reinterpret_cast<volatile unsigned*>(gbase + L::kBar + 16 * kStages + 4);
+  int* prefix = reinterpret_cast<int*>(gbase + L::kPrefix);
+  volatile int* info = reinterpret_cast<volatile int*>(gbase + L::kInfo);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kInfo + 2 * kWarps * 4);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const uint32_t ring = base + warp * kStages * 2 * L::kCodes;
+  const uint32_t bar = base + L::kBar + warp * kStages * 8;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(bar_full + 8 * i, 1);
-      mbar_init(bar_empty + 8 * i, kConsumers / 32);
-    }
-    *abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
+    info[2 * warp] = info[2 * warp + 1] = -1;
     mbar_fence_init();
   }
-  if (warp == 4 && lane == 0) {
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  // prefix[t] = tiles of one row line of the sequences before share t (128
-  // shares of `per` sequences each).
-  auto tiles_of = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kKv8Block - 1) / kKv8Block; };
-  const int per = (p.batch + kConsumers - 1) / kConsumers;
-  if (warp < 4) {
-    long long sum = 0;
+  // prefix[t]: tiles of one line of the sequences before group t (kThreads
+  // groups of `per` sequences).
+  auto tiles_of = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  {
+    int sum = 0;
     for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) sum += tiles_of(b);
-    prefix[threadIdx.x + 1] = sum;
+    int v = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    prefix[threadIdx.x + 1] = v;  // within the warp's 32 groups, for now
     if (threadIdx.x == 0) prefix[0] = 0;
   }
   __syncthreads();
-  if (warp == 0) {
-    long long run = 0;
-    for (int i = 0; i < kConsumers / 32; ++i) {
-      long long v = prefix[1 + i * 32 + lane];
+  int before = 0, all = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      prefix[1 + i * 32 + lane] = v + run;
-      run += __shfl_sync(0xffffffffu, v, 31);
-    }
+  for (int i = 0; i < kWarps; ++i) {
+    const int v = prefix[32 * (i + 1)];
+    if (i < warp) before += v;
+    all += v;
   }
   __syncthreads();
-  const int lines = p.kv_heads * p.row_tiles;  // row lines per sequence
-  const long long total = prefix[kConsumers] * lines;
-  // No more shares than tiles, so that every share has one and arrives where it is counted.
-  const long long grid = max(min(static_cast<long long>(gridDim.x), total), 1LL);
-  auto share_begin = [&](long long i) { return total * i / grid; };
-  const bool idle = blockIdx.x >= grid;
-  const long long u0 = idle ? total : share_begin(blockIdx.x), u1 = idle ? total : share_begin(blockIdx.x + 1LL);
-  // The CTA whose share holds tile u.
-  auto owner = [&](long long u) {
-    long long i = min((u * grid) / total, grid - 1);
-    while (share_begin(i + 1) <= u) ++i;
-    while (share_begin(i) > u) --i;
-    return i;
-  };
-  auto locate = [&](long long u) {
-    int s = 0;  // share of sequences: the last one with prefix * lines <= u
-    for (int step = kConsumers / 2; step > 0; step >>= 1)
-      if (prefix[s + step] * lines <= u) s += step;
+  prefix[threadIdx.x + 1] += before;
+  __syncthreads();
+  const int total = all * p.kv_heads;  // a cache of 2^46 codes has fewer than 2^31 tiles on any GPU
+  // Shares: no more CTAs than tiles, so that every CTA has one and arrives
+  // where it is counted.  The first `more` CTAs take one tile more.
+  const int grid = max(min(static_cast<int>(gridDim.x), total), 1);
+  const int each = total / grid, more = total - each * grid;
+  auto cta_begin = [&](int i) { return i * each + min(i, more); };
+  const bool idle = static_cast<int>(blockIdx.x) >= grid;
+  const int c0 = idle ? total : cta_begin(blockIdx.x), c1 = idle ? total : cta_begin(blockIdx.x + 1);
+  const int u0 = c0 + (c1 - c0) * warp / kWarps, u1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
+  auto locate = [&](int u) {
+    int s = 0;  // the last group with prefix * kv_heads <= u
+#pragma unroll
+    for (int step = kThreads / 2; step > 0; step >>= 1)
+      if (prefix[s + step] * p.kv_heads <= u) s += step;
     Place at;
     at.b = s * per;
-    u -= prefix[s] * lines;
+    int r = u - prefix[s] * p.kv_heads;
     at.tiles = tiles_of(at.b);
-    while (u >= static_cast<long long>(at.tiles) * lines) {
-      u -= static_cast<long long>(at.tiles) * lines;
+    while (r >= at.tiles * p.kv_heads) {
+      r -= at.tiles * p.kv_heads;
       at.tiles = tiles_of(++at.b);
     }
-    at.hr = static_cast<int>(u / at.tiles);
-    at.tile = static_cast<int>(u % at.tiles);
+    at.h = r / at.tiles;
+    at.tile = r - at.h * at.tiles;
     return at;
   };
   // To the next tile; called only when there is one.
   auto advance = [&](Place& at) {
     if (++at.tile < at.tiles) return;
     at.tile = 0;
-    if (++at.hr < lines) return;
-    at.hr = 0;
+    if (++at.h < p.kv_heads) return;
+    at.h = 0;
     do {
       at.tiles = tiles_of(++at.b);
     } while (at.tiles == 0);
   };
-
-  if (warp == 4) {
-    // ------------------------------------------------------------ producer --
-    if (lane == 0 && u0 < u1) {
-      Place at = locate(u0);
-      uint32_t i = 0;
-      for (long long u = u0; u < u1; ++u, ++i) {
-        if (u > u0) advance(at);
-        const uint32_t st = i % kStages;
-        if (!mbar_wait(bar_empty + 8 * st, ((i / kStages) & 1u) ^ 1u, abort_flag, p.status)) break;
-        const uint32_t dst = base + L::kRing + st * 2 * L::kTile;
-        const int head = at.b * p.kv_heads + at.hr / p.row_tiles;
-        mbar_arrive_expect_tx(bar_full + 8 * st, 2 * L::kTile);
-        tma_load_3d(dst, &tm_k, bar_full + 8 * st, 0, at.tile * kKv8Block, head);
-        tma_load_3d(dst + L::kTile, &tm_v, bar_full + 8 * st, 0, at.tile * kKv8Block, head);
-      }
-      // Every copy has landed before the CTA can end: wait for the last use of each stage.
-      for (uint32_t k = i > kStages ? i - kStages : 0; k < i; ++k)
-        mbar_wait_drain(bar_full + 8 * (k % kStages), (k / kStages) & 1u);
-    }
-    return;
-  }
-
-  // ------------------------------------------------------------- consumers --
-  const int g = lane >> 2, c = lane & 3;  // MMA group (row / key / column) and position in it
-  auto sync = [&] { named_bar_sync(1, kConsumers); };
+  auto store8 = [&](int b, int h, int row, int d, const float (&v)[8], float inv) {  // 8 outputs of a row
+    const int tok = row / p.group;
+    const int head = h * p.group + row - tok * p.group;
+    *reinterpret_cast<uint4*>(p.o + b * p.o_batch + tok * p.o_tok + head * p.o_head + d) =
+        make_uint4(pack_half2(v[0] * inv, v[1] * inv), pack_half2(v[2] * inv, v[3] * inv),
+                   pack_half2(v[4] * inv, v[5] * inv), pack_half2(v[6] * inv, v[7] * inv));
+  };
+  // A row without keys has m' = -inf and l = 0 and becomes 0; one with NaN scores has l = NaN.
+  auto inverse = [](float m, float l) { return m == -INFINITY && l == l ? 0.f : 1.f / l; };
   // Rows of sequences without keys.
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (tiles_of(b) > 0) continue;
-    const long long n = static_cast<long long>(p.rows) * p.kv_heads * (HD / 8);
-    for (long long i = threadIdx.x; i < n; i += kConsumers) {
-      const int d8 = static_cast<int>(i % (HD / 8));
-      const long long r = i / (HD / 8);
-      const int head = static_cast<int>(r % (static_cast<long long>(p.kv_heads) * p.group));
-      const long long tok = r / (static_cast<long long>(p.kv_heads) * p.group);
-      *reinterpret_cast<uint4*>(p.o + b * p.o_batch + tok * p.o_tok + head * p.o_head + d8 * 8) = make_uint4(0, 0, 0, 0);
+    const float zero[8] = {};
+    for (int i = threadIdx.x; i < p.rows * p.kv_heads * (HD / 8); i += kThreads) {
+      const int r = i / (HD / 8);
+      store8(b, r / p.rows, r % p.rows, i % (HD / 8) * 8, zero, 0.f);
     }
   }
-  if (u0 >= u1) return;
 
+  const int g = lane >> 2, c = lane & 3;  // MMA group and position in it
   bool ok = true;
-  uint32_t i = 0;
-  Place at = locate(u0);
-  Place nx = at;  // the next tile's place, whose scales are loaded ahead
-  auto scales = [&](const Place& s, float& k, float& v) {
-    const long long idx =
-        (static_cast<long long>(s.b) * p.kv_heads + s.hr / p.row_tiles) * p.n_blocks + s.tile;
-    k = __ldg(p.k_scale + idx);
-    v = __ldg(p.v_scale + idx);
-  };
-  float sk_next, sv_next;
-  scales(at, sk_next, sv_next);
-  for (long long u = u0; u < u1;) {
-    // One sequence's row line: tiles [at.tile, at.tile + count).
-    const int count = static_cast<int>(min(static_cast<long long>(at.tiles - at.tile), u1 - u));
-    const Place seg = at;
-    const int kvh = seg.hr / p.row_tiles;
-    const int r0 = (seg.hr % p.row_tiles) * 16;
-    const int len = kv8_len(p.lens, p.kv_valid, p.kv_len, seg.b);
-    uint32_t qf[HD / 16][4];
-    int lim[2];  // keys visible to rows g and g + 8
+  if (u0 < u1) {
+    // ------------------------------------------------------- the warp's share --
+    Place at = locate(u0);
+    Place ahead = at;  // the next tile to load (lane 0)
+    int ua = u0;
+    auto load = [&](uint32_t st) {
+      if (ua > u0) advance(ahead);
+      ++ua;
+      const uint32_t dst = ring + st * 2 * L::kCodes;
+      const int head = ahead.b * p.kv_heads + ahead.h;
+      mbar_arrive_expect_tx(bar + 8 * st, 2 * L::kCodes);
+      tma_load_3d(dst, &tm_k, bar + 8 * st, 0, ahead.tile * kTileKeys, head);
+      tma_load_3d(dst + L::kCodes, &tm_v, bar + 8 * st, 0, ahead.tile * kTileKeys, head);
+    };
+    if (lane == 0)
+      for (int i = 0; i < kStages && ua < u1; ++i) load(i);
+    auto scales = [&](const Place& s, float& k, float& v) {
+      const long long idx =
+          (static_cast<long long>(s.b) * p.kv_heads + s.h) * p.n_blocks + s.tile / (kKv8Block / kTileKeys);
+      k = __ldg(p.k_scale + idx);
+      v = __ldg(p.v_scale + idx);
+    };
+    Place nx = at;  // the next tile's place, whose scales are loaded ahead
+    float sk_next, sv_next;
+    scales(at, sk_next, sv_next);
+    uint32_t st = 0, ph = 0;
+    for (int u = u0; u < u1;) {
+      // One line's tiles [at.tile, at.tile + count).
+      const Place seg = at;
+      const int count = min(seg.tiles - seg.tile, u1 - u);
+      const int len = kv8_len(p.lens, p.kv_valid, p.kv_len, seg.b);
+      const int line0 = u - seg.tile;
+      uint32_t qf[NT][HD / 16][2];
+      int lim[NT][2];  // keys visible to rows 8 nt + 2c and the next
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = r0 + g + 8 * x;
-      lim[x] = 0;
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) qf[k][x] = qf[k][x + 2] = 0u;
-      if (r < p.rows) {
-        const int tok = r / p.group;
-        const int head = kvh * p.group + r % p.group;
-        lim[x] = p.causal ? min(len, len - p.q_len + tok + 1) : len;
-        // This lane's k indexes: HD / 4 consecutive values of the row; MMA step k takes four of them.
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + tok * p.q_tok + head * p.q_head +
-                                                          c * (HD / 4));
-#pragma unroll
-        for (int k = 0; k < HD / 32; ++k) {
-          const uint4 v = __ldg(src + k);
-          qf[2 * k][x] = v.x;
-          qf[2 * k][x + 2] = v.y;
-          qf[2 * k + 1][x] = v.z;
-          qf[2 * k + 1][x + 2] = v.w;
-        }
-      }
-    }
-    float acc[HD / 8][4];
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int t = 0; t < count; ++t, ++u, ++i) {
-      const float sk = sk_next, sv = sv_next;
-      at = nx;
-      if (u + 1 < u1) {
-        advance(nx);
-        scales(nx, sk_next, sv_next);
-      }
-      const uint32_t st = i % kStages;
-      if (ok) ok = mbar_wait_warp(bar_full + 8 * st, (i / kStages) & 1u, abort_flag, p.status);
-      if (!ok) continue;
-      const uint32_t kt = base + L::kRing + st * 2 * L::kTile, vt = kt + L::kTile;
-      // K rows of the warp's 16 keys (8 per MMA column tile).
-      uint32_t kw[2][HD / 16];
-#pragma unroll
-      for (int n8 = 0; n8 < 2; ++n8) {
-        const int key = warp * 16 + n8 * 8 + g;
-#pragma unroll
-        for (int k = 0; k < HD / 64; ++k) {
-          // 16-byte run c * (HD / 64) + k of the row, at its swizzled place.
-          const int run = c * (HD / 64) + k;
-          const int at16 = HD == 128 ? run ^ (key & 7) : run ^ ((key >> 1) & 3);
-          const uint4 v = ld_shared_v4u(kt + key * HD + at16 * 16);
-          kw[n8][4 * k] = v.x;
-          kw[n8][4 * k + 1] = v.y;
-          kw[n8][4 * k + 2] = v.z;
-          kw[n8][4 * k + 3] = v.w;
-        }
-      }
-      // V: HD / 8 codes of each of the lane's four keys 2c, 2c + 1, 2c + 8, 2c + 9.
-      uint32_t vw[4][HD / 32];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = warp * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
-        if constexpr (HD == 128) {
-          const uint4 v = ld_shared_v4u(vt + key * HD + ((g ^ (key & 7)) << 4));
-          vw[x][0] = v.x;
-          vw[x][1] = v.y;
-          vw[x][2] = v.z;
-          vw[x][3] = v.w;
-        } else {
-          const uint2 v = ld_shared_v2u(vt + key * HD + (((g >> 1) ^ ((key >> 1) & 3)) << 4) + (g & 1) * 8);
-          vw[x][0] = v.x;
-          vw[x][1] = v.y;
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_empty + 8 * st);  // the stage is in registers
-      float s[2][4];
-#pragma unroll
-      for (int n8 = 0; n8 < 2; ++n8) {
-        s[n8][0] = s[n8][1] = s[n8][2] = s[n8][3] = 0.f;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          uint32_t b0, b1;
-          kv8_to_half2<FMT>(kw[n8][k], b0, b1);
-          mma_16816(s[n8], qf[k], b0, b1);
-        }
-      }
-      // A block whose K scale is 0 has only zero codes: any factor gives its
-      // scores, 0; 1 keeps a masked -inf from meeting 0.
-      const float mul = sk > 0.f ? sk * p.scale_log2 : 1.f;
-      const float lsv = sv > 0.f ? __log2f(sv) : kNoScale;
-      const float isv = sv > 0.f ? __fdividef(1.f, sv) : 8589934592.f;  // 2^33
-      const int key0 = at.tile * kKv8Block + warp * 16 + 2 * c;
-      const bool edge = at.tile * kKv8Block + kKv8Block > min(len, p.causal ? len - p.q_len + 1 : len);
-      if (edge) {
-#pragma unroll
-        for (int n8 = 0; n8 < 2; ++n8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key0 + n8 * 8 + (e & 1) >= lim[e >> 1]) s[n8][e] = -INFINITY;
-        if constexpr (FMT == kKv8E4m3) {
-          // What lies past the length may decode to NaN, and 0 * NaN is NaN.
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (key0 + (x & 1) + (x >> 1) * 8 >= len) {
-#pragma unroll
-              for (int k = 0; k < HD / 32; ++k) vw[x][k] = 0u;
-            }
-        }
-      }
-      bool grow = false;
-      float top[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float mx = fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        top[x] = fmaf(mx, mul, lsv);
-        grow |= top[x] > m[x] + kRescale;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        // The maximum moves, and what is summed so far with it, only when it
-        // would otherwise lag by more than 2^8 (fp16 holds p' up to 2^16).
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float mn = fmaxf(m[x], top[x]);
-          const float f = mn == m[x] ? 1.f : ex2_approx(m[x] - mn);
-          m[x] = mn;
-          l[x] *= f;
+          const int r = 8 * nt + 2 * c + x;
+          lim[nt][x] = p.causal && r < p.rows ? min(len, len - p.q_len + r / p.group + 1) : len;
+        }
+        const int r = 8 * nt + g;
 #pragma unroll
-          for (int j = 0; j < HD / 8; ++j) {
-            acc[j][2 * x] *= f;
-            acc[j][2 * x + 1] *= f;
+        for (int k = 0; k < HD / 16; ++k) qf[nt][k][0] = qf[nt][k][1] = 0u;
+        if (r < p.rows) {
+          const int tok = r / p.group;
+          const int head = seg.h * p.group + r - tok * p.group;
+          // This lane's k indexes: HD / 4 consecutive values of the row, four of them in each MMA step.
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + tok * p.q_tok + head * p.q_head +
+                                                            c * (HD / 4));
+#pragma unroll
+          for (int k = 0; k < HD / 32; ++k) {
+            const uint4 v = __ldg(src + k);
+            qf[nt][2 * k][0] = v.x;
+            qf[nt][2 * k][1] = v.y;
+            qf[nt][2 * k + 1][0] = v.z;
+            qf[nt][2 * k + 1][1] = v.w;
           }
         }
       }
-      uint32_t pf[4];
+      float acc[NT][HD / 16][4];
+      float m[NT][2], l[NT][2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float off = lsv - (m[x] == -INFINITY ? 0.f : m[x]);
-        float sum = 0.f;
+      for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-        for (int n8 = 0; n8 < 2; ++n8) {
-          const float a = ex2_approx(fmaf(s[n8][2 * x], mul, off));
-          const float b = ex2_approx(fmaf(s[n8][2 * x + 1], mul, off));
-          sum += a + b;
-          pf[2 * n8 + x] = pack_half2(a, b);
+        for (int j = 0; j < HD / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
+      }
+      // Keys from here on are hidden from some row.
+      const int edge = min(len, p.causal ? len - p.q_len + 1 : len);
+      for (int t = 0; t < count; ++t, ++u) {
+        const float sk = sk_next, sv = sv_next;
+        const int key0 = nx.tile * kTileKeys;
+        if (u + 1 < u1) {
+          advance(nx);
+          scales(nx, sk_next, sv_next);
         }
-        l[x] = fmaf(sum, isv, l[x]);
-      }
-      // O' += P V: MMA j takes code j of every lane's run, so its columns are d = (HD / 8) n + j.
+        if (ok) ok = mbar_wait_warp(bar + 8 * st, ph, abort_flag, p.status);
+        if (!ok) continue;
+        const uint32_t kt = ring + st * 2 * L::kCodes, vt = kt + L::kCodes;
+        // K: the lane's runs of rows 16 i + g and 16 i + g + 8.
+        uint32_t kw[2][2][HD / 16];
 #pragma unroll
-      for (int k = 0; k < HD / 32; ++k) {
-        const uint32_t a0 = prmt(vw[0][k], vw[1][k], 0x5140u), a1 = prmt(vw[0][k], vw[1][k], 0x7362u);
-        const uint32_t c0 = prmt(vw[2][k], vw[3][k], 0x5140u), c1 = prmt(vw[2][k], vw[3][k], 0x7362u);
-        uint32_t lo0, lo1, lo2, lo3, hi0, hi1, hi2, hi3;
-        kv8_to_half2<FMT>(a0, lo0, lo1);
-        kv8_to_half2<FMT>(a1, lo2, lo3);
-        kv8_to_half2<FMT>(c0, hi0, hi1);
-        kv8_to_half2<FMT>(c1, hi2, hi3);
-        mma_16816(acc[4 * k], pf, lo0, hi0);
-        mma_16816(acc[4 * k + 1], pf, lo1, hi1);
-        mma_16816(acc[4 * k + 2], pf, lo2, hi2);
-        mma_16816(acc[4 * k + 3], pf, lo3, hi3);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int key = 16 * i + 8 * x + g;
+#pragma unroll
+            for (int k = 0; k < HD / 64; ++k) {
+              const int run = c * (HD / 64) + k;
+              const int at16 = HD == 128 ? run ^ (key & 7) : run ^ ((key >> 1) & 3);
+              const uint4 v = ld_shared_v4u(kt + key * HD + at16 * 16);
+              kw[i][x][4 * k] = v.x;
+              kw[i][x][4 * k + 1] = v.y;
+              kw[i][x][4 * k + 2] = v.z;
+              kw[i][x][4 * k + 3] = v.w;
+            }
+          }
+        // V: HD / 8 codes of each of the lane's keys 16 i + 2c, + 1, + 8, + 9.
+        uint32_t vw[2][4][HD / 32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = 16 * i + 2 * c + (x & 1) + (x >> 1) * 8;
+            if constexpr (HD == 128) {
+              const uint4 v = ld_shared_v4u(vt + key * HD + ((g ^ (key & 7)) << 4));
+              vw[i][x][0] = v.x;
+              vw[i][x][1] = v.y;
+              vw[i][x][2] = v.z;
+              vw[i][x][3] = v.w;
+            } else {
+              const uint2 v = ld_shared_v2u(vt + key * HD + (((g >> 1) ^ ((key >> 1) & 3)) << 4) + (g & 1) * 8);
+              vw[i][x][0] = v.x;
+              vw[i][x][1] = v.y;
+            }
+          }
+        // The tile is in registers: its stage takes the next load.
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && ua < u1) load(st);
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1u;
+        }
+        float s[NT][2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[nt][i][0] = s[nt][i][1] = s[nt][i][2] = s[nt][i][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a0, a1, a2, a3;
+            kv8_to_half2<FMT>(kw[i][0][k], a0, a2);
+            kv8_to_half2<FMT>(kw[i][1][k], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][i], a0, a1, a2, a3, qf[nt][k][0], qf[nt][k][1]);
+          }
+        // A block whose K scale is 0 has only zero codes: any factor gives its
+        // scores, 0; 1 keeps a masked -inf from meeting 0.
+        const float mul = sk > 0.f ? sk * p.scale_log2 : 1.f;
+        const float lsv = sv > 0.f ? __log2f(sv) : kNoScale;
+        const float isv = sv > 0.f ? __fdividef(1.f, sv) : 8589934592.f;  // 2^33
+        if (key0 + kTileKeys > edge) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key0 + 16 * i + 8 * (e >> 1) + g >= lim[nt][e & 1]) s[nt][i][e] = -INFINITY;
+          if constexpr (FMT == kKv8E4m3) {
+            // What lies past the length may decode to NaN, and 0 * NaN is NaN.
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (key0 + 16 * i + 2 * c + (x & 1) + (x >> 1) * 8 >= len) {
+#pragma unroll
+                  for (int k = 0; k < HD / 32; ++k) vw[i][x][k] = 0u;
+                }
+          }
+        }
+        bool grow = false;
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float mx = fmaxf(fmaxf(s[nt][0][x], s[nt][0][2 + x]), fmaxf(s[nt][1][x], s[nt][1][2 + x]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            top[nt][x] = fmaf(mx, mul, lsv);
+            grow |= top[nt][x] > m[nt][x] + kRescale;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+          // The maximum moves, and what is summed so far with it, only when it
+          // would otherwise lag by more than 2^8 (fp16 holds p' up to 2^16).
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float mn = fmaxf(m[nt][x], top[nt][x]);
+              const float f = mn == m[nt][x] ? 1.f : ex2_approx(m[nt][x] - mn);
+              m[nt][x] = mn;
+              l[nt][x] *= f;
+#pragma unroll
+              for (int j = 0; j < HD / 16; ++j) {
+                acc[nt][j][x] *= f;
+                acc[nt][j][2 + x] *= f;
+              }
+            }
+        }
+        uint32_t pf[NT][2][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float off[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) off[x] = lsv - (m[nt][x] == -INFINITY ? 0.f : m[nt][x]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float a = ex2_approx(fmaf(s[nt][i][2 * y], mul, off[0]));
+              const float b = ex2_approx(fmaf(s[nt][i][2 * y + 1], mul, off[1]));
+              sum[0] += a;
+              sum[1] += b;
+              pf[nt][i][y] = transpose8(pack_half2(a, b));
+            }
+          l[nt][0] = fmaf(sum[0], isv, l[nt][0]);
+          l[nt][1] = fmaf(sum[1], isv, l[nt][1]);
+        }
+        // O'^T += V^T P^T: MMA j takes codes 2j and 2j + 1 of every lane's run.
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < HD / 32; ++k)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t sel = y == 0 ? 0x5140u : 0x7362u;  // codes 0, 1 / 2, 3 of two keys, interleaved
+              uint32_t a0, a1, a2, a3;
+              kv8_to_half2<FMT>(prmt(vw[i][0][k], vw[i][1][k], sel), a0, a1);
+              kv8_to_half2<FMT>(prmt(vw[i][2][k], vw[i][3][k], sel), a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][2 * k + y], a0, a1, a2, a3, pf[nt][i][0], pf[nt][i][1]);
+            }
       }
+      at = nx;
+      // The line's sums over the lanes of a column; then out, or into a slot.
+      const bool whole = seg.tile == 0 && count == seg.tiles;
+      const bool first = line0 + seg.tile == u0;  // the share's first line
+      float* slot = reinterpret_cast<float*>(gbase + (first ? L::kHead + warp * L::kSlot : ring - base));
+      if (!whole && !first) __syncwarp();  // the ring's last tile has been read by all lanes
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float sum = l[nt][x];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = 8 * nt + 2 * c + x;
+          if (row < p.rows) {
+            if (whole) {
+              const float inv = inverse(m[nt][x], sum);
+#pragma unroll
+              for (int j = 0; j < HD / 16; j += 4) {
+                const float v[8] = {acc[nt][j][x],     acc[nt][j][2 + x],     acc[nt][j + 1][x], acc[nt][j + 1][2 + x],
+                                    acc[nt][j + 2][x], acc[nt][j + 2][2 + x], acc[nt][j + 3][x], acc[nt][j + 3][2 + x]};
+                if (ok) store8(seg.b, seg.h, row, g * (HD / 8) + 2 * j, v, inv);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < HD / 16; j += 2)
+                reinterpret_cast<float4*>(slot)[row * kF4 + g * (HD / 32) + j / 2] =
+                    make_float4(acc[nt][j][x], acc[nt][j][2 + x], acc[nt][j + 1][x], acc[nt][j + 1][2 + x]);
+              if (g == 0) {
+                slot[L::kRows * HD + row] = m[nt][x];
+                slot[L::kRows * HD + L::kRows + row] = sum;
+              }
+            }
+          }
+        }
+      if (!whole && lane == 0 && ok) info[2 * warp + (first ? 0 : 1)] = line0;
     }
-    at = nx;
+    // On a timeout, loads of this warp may still be landing.
+    if (!ok && lane == 0)
+      for (int i = 0; i < kStages; ++i) mbar_wait_drain(bar + 8 * i, ph ^ (i < static_cast<int>(st) ? 1u : 0u));
+  }
+  __syncthreads();
+  if (*abort_flag != 0 || c0 >= c1) return;
 
-    // Join the four warps' parts: rows' maxima and sums first, then O'.
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (c == 0) {
-        stat[(warp * 16 + g + 8 * x) * 2] = m[x];
-        stat[(warp * 16 + g + 8 * x) * 2 + 1] = l[x];
+  // ------------------------------------------- lines that cross warps or CTAs --
+  // Slots in order (first and last line of warp 0, of warp 1, ...); runs of
+  // slots of one line (kWarps + 1 at most) are dealt to the warps.
+  for (int mine_run = warp; mine_run <= kWarps; mine_run += kWarps) {
+    int run = -1, s0 = -1, s1 = -1, last_line = -1, line = -1;
+    for (int i = 0; i < 2 * kWarps; ++i) {
+      const int li = info[i];
+      if (li < 0) continue;
+      if (li != last_line) ++run;
+      last_line = li;
+      if (run == mine_run) {
+        if (s0 < 0) s0 = i;
+        s1 = i;
+        line = li;
       }
     }
-    sync();
-    float* merge = reinterpret_cast<float*>(gbase + L::kMerge);
-    // 16-byte unit f of row r is kept at unit f ^ mix(f, r), which spreads a
-    // quarter warp's stores over the banks.
-    auto unit = [](int r, int f) {
-      const int mix = HD == 128 ? ((f >> 3) & 3) | ((r & 1) << 2) : ((f >> 3) & 1) | ((r & 1) << 1);
-      return r * (HD / 4) + (f ^ mix);
-    };
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = g + 8 * x;
-      float mm = m[x];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, stat[(w * 16 + r) * 2]);
-      const float f = m[x] == mm ? 1.f : ex2_approx(m[x] - mm);
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int j = 0; j < HD / 8; j += 4) {
-          const float4 v = make_float4(acc[j][2 * x + half] * f, acc[j + 1][2 * x + half] * f,
-                                       acc[j + 2][2 * x + half] * f, acc[j + 3][2 * x + half] * f);
-          const int f4 = ((2 * c + half) * (HD / 8) + j) / 4;
-          reinterpret_cast<float4*>(merge)[warp * 16 * (HD / 4) + unit(r, f4)] = v;
-        }
-    }
-    sync();
-    const bool whole = count == seg.tiles;
-    const long long line0 = u - count - seg.tile;  // the line's first tile
-    float* slot = p.part + (2LL * blockIdx.x + (u - count == u0 ? 0 : 1)) * (16 * HD + 32);
-    const int rows_here = min(16, p.rows - r0);
-    auto store = [&](int r, int f4, float4 v, float inv) {
-      const int row = r0 + r;
-      const int tok = row / p.group;
-      const int head = kvh * p.group + row % p.group;
-      *reinterpret_cast<uint2*>(p.o + seg.b * p.o_batch + tok * p.o_tok + head * p.o_head + f4 * 4) =
+    if (s0 < 0) break;
+    const Place at = locate(line);
+    const bool inside = line >= c0 && line + at.tiles <= c1;
+    auto put = [&](int e, const float4& v, float inv) {
+      const int r = e / kF4;
+      const int tok = r / p.group;
+      const int head = at.h * p.group + r - tok * p.group;
+      *reinterpret_cast<uint2*>(p.o + at.b * p.o_batch + tok * p.o_tok + head * p.o_head + e % kF4 * 4) =
           make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
     };
-    // A row without keys has m' = -inf and l = 0 and becomes 0; one with NaN scores has l = NaN.
-    auto inverse = [](float mm, float ll) { return mm == -INFINITY && ll == ll ? 0.f : 1.f / ll; };
-    if (ok) {
-      for (int e = threadIdx.x; e < rows_here * (HD / 4); e += kConsumers) {
-        const int r = e / (HD / 4), f4 = e % (HD / 4);
-        float mm = -INFINITY, ll = 0.f;
+    // Joins parts k0..k1 (get(k): O', m', l of unit e) in order, eight loads at a time.
+    auto join = [&](int e, int k0, int k1, auto get, float4& v, float& m, float& l) {
+      m = -INFINITY;
+      l = 0.f;
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = k0; k <= k1; k += 8) {
+        float4 o[8];
+        float pm[8], pl[8];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, stat[(w * 16 + r) * 2]);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float mw = stat[(w * 16 + r) * 2];
-          ll += stat[(w * 16 + r) * 2 + 1] * (mw == mm ? 1.f : ex2_approx(mw - mm));
-          const float4 o = reinterpret_cast<const float4*>(merge)[w * 16 * (HD / 4) + unit(r, f4)];
-          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        for (int i = 0; i < 8; ++i) {
+          pm[i] = -INFINITY;
+          pl[i] = 0.f;
+          o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k + i <= k1) get(k + i, e, o[i], pm[i], pl[i]);
         }
-        if (whole) {
-          store(r, f4, v, inverse(mm, ll));
-        } else {
-          reinterpret_cast<float4*>(slot + 32)[r * (HD / 4) + f4] = v;
-          if (f4 == 0) {
-            slot[r] = mm;
-            slot[16 + r] = ll;
-          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float mn = fmaxf(m, pm[i]);
+          const float fo = m == mn ? 1.f : ex2_approx(m - mn);
+          const float fn = pm[i] == mn ? 1.f : ex2_approx(pm[i] - mn);
+          m = mn;
+          l = l * fo + pl[i] * fn;
+          v = make_float4(v.x * fo + o[i].x * fn, v.y * fo + o[i].y * fn, v.z * fo + o[i].z * fn, v.w * fo + o[i].w * fn);
+        }
+      }
+    };
+    auto in_shared = [&](int k, int e, float4& o, float& pm, float& pl) {
+      if (info[k] != line) return;
+      const float* s = reinterpret_cast<const float*>(
+          gbase + ((k & 1) ? static_cast<uint32_t>(k >> 1) * kStages * 2 * L::kCodes : L::kHead + (k >> 1) * L::kSlot));
+      pm = s[L::kRows * HD + e / kF4];
+      pl = s[L::kRows * HD + L::kRows + e / kF4];
+      o = reinterpret_cast<const float4*>(s)[e];
+    };
+    constexpr int kPart = L::kSlot / 4;
+    float* mine = p.part + (2LL * blockIdx.x + (line <= c0 ? 0 : 1)) * kPart;  // one part per end of the CTA's share
+    for (int e = lane; e < p.rows * kF4; e += 32) {
+      float4 v;
+      float m, l;
+      join(e, s0, s1, in_shared, v, m, l);
+      if (inside) {
+        put(e, v, inverse(m, l));
+      } else {
+        reinterpret_cast<float4*>(mine)[e] = v;
+        if (e % kF4 == 0) {
+          mine[L::kRows * HD + e / kF4] = m;
+          mine[L::kRows * HD + L::kRows + e / kF4] = l;
         }
       }
     }
-    if (!whole) {
-      // Count in; the last part of the line joins them all, in CTA order.
-      __threadfence();
-      sync();
-      const long long first = owner(line0), last = owner(line0 + seg.tiles - 1);
-      unsigned* count_at = p.count + static_cast<long long>(seg.b) * lines + seg.hr;
-      if (threadIdx.x == 0) {
-        const unsigned n = static_cast<unsigned>(last - first + 1);
-        const unsigned before = ok ? atomicAdd(count_at, 1u) : 0u;
-        *last_flag = ok && before == n - 1 ? 1u : 0u;
-        if (ok && before == n - 1) *count_at = 0u;  // ready for the next launch
-      }
-      sync();
-      if (*last_flag != 0u) {
-        __threadfence();
-        for (int e = threadIdx.x; e < rows_here * (HD / 4); e += kConsumers) {
-          const int r = e / (HD / 4), f4 = e % (HD / 4);
-          float mm = -INFINITY, ll = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (long long k = first; k <= last; ++k) {
-            // A part that does not start its CTA's share can only be the first.
-            const float* part = p.part + (2 * k + (k == first && share_begin(k) != line0 ? 1 : 0)) * (16 * HD + 32);
-            const float pm = __ldcg(part + r), pl = __ldcg(part + 16 + r);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(part + 32) + r * (HD / 4) + f4);
-            const float mn = fmaxf(mm, pm);
-            const float fo = mm == mn ? 1.f : ex2_approx(mm - mn);
-            const float fn = pm == mn ? 1.f : ex2_approx(pm - mn);
-            mm = mn;
-            ll = ll * fo + pl * fn;
-            v = make_float4(v.x * fo + o.x * fn, v.y * fo + o.y * fn, v.z * fo + o.z * fn, v.w * fo + o.w * fn);
-          }
-          store(r, f4, v, inverse(mm, ll));
-        }
-      }
+    if (inside) continue;
+    // Count in; the last part of the line joins them all, in CTA order.
+    auto owner = [&](int u) {  // the CTA whose share holds tile u
+      const int big = more * (each + 1);
+      return u < big ? u / (each + 1) : more + (u - big) / each;
+    };
+    const int first = owner(line), last = owner(line + at.tiles - 1);
+    __threadfence();
+    __syncwarp();
+    unsigned n = 0;
+    unsigned* count = p.count + static_cast<long long>(at.b) * p.kv_heads + at.h;
+    if (lane == 0) {
+      n = atomicAdd(count, 1u) + 1u;
+      if (n == static_cast<unsigned>(last - first + 1)) *count = 0u;  // ready for the next launch
     }
-    sync();  // merge and stat are free again
+    n = __shfl_sync(0xffffffffu, n, 0);
+    if (n != static_cast<unsigned>(last - first + 1)) continue;
+    __threadfence();
+    // Only the first part may lie behind its CTA's first tile.
+    const int first_slot = line <= cta_begin(first) ? 0 : 1;
+    auto in_global = [&](int k, int e, float4& o, float& pm, float& pl) {
+      const float* s = p.part + (2LL * k + (k == first ? first_slot : 0)) * kPart;
+      pm = __ldcg(s + L::kRows * HD + e / kF4);
+      pl = __ldcg(s + L::kRows * HD + L::kRows + e / kF4);
+      o = __ldcg(reinterpret_cast<const float4*>(s) + e);
+    };
+    for (int e = lane; e < p.rows * kF4; e += 32) {
+      float4 v;
+      float m, l;
+      join(e, first, last, in_global, v, m, l);
+      put(e, v, inverse(m, l));
+    }
   }
 }
 
-template <int FMT, int HD>
-cudaError_t launch_hd(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
+template <int FMT, int HD, int NT>
+cudaError_t launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
                       cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
   const uint64_t bit = 1ull << (dev & 63);
-  auto kernel = kv8_rows_sm100_kernel<FMT, HD>;
+  auto kernel = kv8_rows_sm100_kernel<FMT, HD, NT>;
   if ((configured.load(std::memory_order_acquire) & bit) == 0) {
     const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<HD>::kBytes);
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<HD, NT>::kBytes);
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
-  kernel<<<grid, kThreads, RowsSmem<HD>::kBytes, stream>>>(tk, tv, p);
+  kernel<<<grid, kThreads, RowsSmem<HD, NT>::kBytes, stream>>>(tk, tv, p);
   return cudaGetLastError();
+}
+template <int FMT, int HD>
+cudaError_t launch_hd(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
+                      cudaStream_t stream) {
+  return p.rows <= 8 ? launch_nt<FMT, HD, 1>(tk, tv, p, grid, dev, stream)
+                     : launch_nt<FMT, HD, 2>(tk, tv, p, grid, dev, stream);
 }
 
 }  // namespace
 
-// Two CTAs per SM, but none without a tile when every sequence is as long as it can be.
+// One CTA per SM, but none without a tile when every sequence is as long as it can be.
 int kv8_rows_grid(const Kv8AttnParams& p, int sms) {
-  const long long tiles = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles *
-                          ((p.kv_len + kKv8Block - 1) / kKv8Block);
-  const long long most = static_cast<long long>(kCtasPerSm) * sms;
-  return static_cast<int>(tiles < most ? (tiles > 0 ? tiles : 1) : most);
+  const long long tiles =
+      static_cast<long long>(p.batch) * p.kv_heads * ((p.kv_len + kTileKeys - 1) / kTileKeys);
+  return static_cast<int>(tiles < sms ? (tiles > 0 ? tiles : 1) : sms);
 }
-size_t kv8_rows_part_floats(int head_dim, int grid) { return 2 * static_cast<size_t>(grid) * (16 * head_dim + 32); }
+int kv8_rows_tile() { return kTileKeys; }
+size_t kv8_rows_part_floats(int head_dim, int grid) { return 2 * static_cast<size_t>(grid) * 16 * (head_dim + 2); }
 
 cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
                             cudaStream_t stream) {
