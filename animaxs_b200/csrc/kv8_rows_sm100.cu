@@ -48,6 +48,11 @@ constexpr int kTileKeys = 32;
 constexpr float kRescale = 8.f;    // log2 units by which the maximum may lag
 constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
+// What a slot holds: the line's first tile (-1: nothing), sequence, kv head and tiles.
+struct alignas(16) SlotInfo {
+  int line, b, h, tiles;
+};
+
 // NT: column tiles of 8 query rows (1 or 2).
 template <int HD, int NT>
 struct RowsSmem {
@@ -59,8 +64,8 @@ struct RowsSmem {
   static constexpr uint32_t kHead = kRing;                        // [warp] part of the share's first line
   static constexpr uint32_t kPrefix = kHead + kWarps * kSlot;     // int32 [kThreads + 1]
   static constexpr uint32_t kBar = (kPrefix + (kThreads + 1) * 4 + 15) / 16 * 16;
-  static constexpr uint32_t kInfo = kBar + kWarps * kStages * 8;  // int [2 * warp]: line of the slot, -1: none
-  static constexpr uint32_t kBytes = kInfo + 2 * kWarps * 4 + 16 + 1024;  // + alignment slack
+  static constexpr uint32_t kInfo = (kBar + kWarps * kStages * 8 + 15) / 16 * 16;  // SlotInfo [2 * warp]
+  static constexpr uint32_t kBytes = kInfo + 2 * kWarps * 16 + 16 + 1024;  // + alignment slack
   // The part of a share's last line goes to the warp's own ring, which is idle by then.
   static_assert(kStages * 2 * kCodes >= kSlot, "a slot must fit a warp's ring");
   static_assert(kBytes <= 227 * 1024, "shared memory exceeds the 227 KiB opt-in");
@@ -110,50 +115,49 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   int* prefix = reinterpret_cast<int*>(gbase + L::kPrefix);
-  volatile int* info = reinterpret_cast<volatile int*>(gbase + L::kInfo);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kInfo + 2 * kWarps * 4);
+  SlotInfo* info = reinterpret_cast<SlotInfo*>(gbase + L::kInfo);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kInfo + 2 * kWarps * 16);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t ring = base + warp * kStages * 2 * L::kCodes;
   const uint32_t bar = base + L::kBar + warp * kStages * 8;
 
+  // prefix[t]: tiles of one line of the sequences before group t (kThreads
+  // groups of `per` sequences).
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  auto tiles_in = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
+  int scan = 0;
+  for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) scan += tiles_in(b);
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
-    info[2 * warp] = info[2 * warp + 1] = -1;
+    info[2 * warp].line = info[2 * warp + 1].line = -1;
     mbar_fence_init();
   }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
+    prefix[0] = 0;
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  // prefix[t]: tiles of one line of the sequences before group t (kThreads
-  // groups of `per` sequences).
-  auto tiles_of = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  {
-    int sum = 0;
-    for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) sum += tiles_of(b);
-    int v = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    prefix[threadIdx.x + 1] = v;  // within the warp's 32 groups, for now
-    if (threadIdx.x == 0) prefix[0] = 0;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += u;
   }
+  int* warp_sum = reinterpret_cast<int*>(gbase + L::kHead);  // free until a share ends
+  if (lane == 31) warp_sum[warp] = scan;
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) {
-    const int v = prefix[32 * (i + 1)];
+    const int v = warp_sum[i];
     if (i < warp) before += v;
     all += v;
   }
+  prefix[threadIdx.x + 1] = scan + before;
   __syncthreads();
-  prefix[threadIdx.x + 1] += before;
-  __syncthreads();
+  // Up to kThreads sequences their tiles are in shared memory.
+  auto tiles_of = [&](int b) { return per == 1 ? prefix[b + 1] - prefix[b] : tiles_in(b); };
   const int total = all * p.kv_heads;  // a cache of 2^46 codes has fewer than 2^31 tiles on any GPU
   // Shares: no more CTAs than tiles, so that every CTA has one and arrives
   // where it is counted.  The first `more` CTAs take one tile more.
@@ -163,11 +167,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool idle = static_cast<int>(blockIdx.x) >= grid;
   const int c0 = idle ? total : cta_begin(blockIdx.x), c1 = idle ? total : cta_begin(blockIdx.x + 1);
   const int u0 = c0 + (c1 - c0) * warp / kWarps, u1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
-  auto locate = [&](int u) {
-    int s = 0;  // the last group with prefix * kv_heads <= u
-#pragma unroll
-    for (int step = kThreads / 2; step > 0; step >>= 1)
-      if (prefix[s + step] * p.kv_heads <= u) s += step;
+  static_assert(kThreads == 256, "locate() searches 32 x 8 groups");
+  auto locate = [&](int u) {  // by a converged warp
+    // The last group with prefix * kv_heads <= u: by eights, then one by one.
+    int s = 8 * __popc(__ballot_sync(0xffffffffu, prefix[8 * (lane + 1)] * p.kv_heads <= u));
+    s += __popc(__ballot_sync(0xffffffffu, lane < 8 && prefix[s + (lane & 7) + 1] * p.kv_heads <= u));
     Place at;
     at.b = s * per;
     int r = u - prefix[s] * p.kv_heads;
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-      if (!whole && lane == 0 && ok) info[2 * warp + (first ? 0 : 1)] = line0;
+      if (!whole && lane == 0 && ok) info[2 * warp + (first ? 0 : 1)] = SlotInfo{line0, seg.b, seg.h, seg.tiles};
     }
     // On a timeout, loads of this warp may still be landing.
     if (!ok && lane == 0)
@@ -488,112 +492,130 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (*abort_flag != 0 || c0 >= c1) return;
 
   // ------------------------------------------- lines that cross warps or CTAs --
-  // Slots in order (first and last line of warp 0, of warp 1, ...); runs of
-  // slots of one line (kWarps + 1 at most) are dealt to the warps.
-  for (int mine_run = warp; mine_run <= kWarps; mine_run += kWarps) {
-    int run = -1, s0 = -1, s1 = -1, last_line = -1, line = -1;
-    for (int i = 0; i < 2 * kWarps; ++i) {
-      const int li = info[i];
-      if (li < 0) continue;
-      if (li != last_line) ++run;
-      last_line = li;
-      if (run == mine_run) {
-        if (s0 < 0) s0 = i;
-        s1 = i;
-        line = li;
+  // Slots in order (first and last line of warp 0, of warp 1, ...); the slots of
+  // one line are a run.  Warp 0 lists the runs: mask of the slots, and in
+  // ends[0] / ends[1] the line that goes on before / behind the CTA's share.
+  // All code from here on runs once, out of a cold instruction cache, so it is
+  // kept small rather than unrolled.
+  uint32_t* runs = reinterpret_cast<uint32_t*>(prefix);          // [kWarps + 1]
+  int* ends = prefix + kWarps + 2;                               // slot index of the line, -1: none
+  volatile int* n_runs = prefix + kWarps + 4;
+  const int units = p.rows * kF4;
+  constexpr int kPart = L::kSlot / 4;
+  auto put = [&](const SlotInfo& at, int e, const float4& v, float m, float l) {
+    const float inv = inverse(m, l);
+    const int r = e / kF4;
+    const int tok = r / p.group;
+    const int head = at.h * p.group + r - tok * p.group;
+    *reinterpret_cast<uint2*>(p.o + at.b * p.o_batch + tok * p.o_tok + head * p.o_head + e % kF4 * 4) =
+        make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+  };
+  auto add_part = [](float4& v, float& m, float& l, const float4& o, float pm, float pl) {
+    const float mn = fmaxf(m, pm);
+    const float fo = m == mn ? 1.f : ex2_approx(m - mn);
+    const float fn = pm == mn ? 1.f : ex2_approx(pm - mn);
+    m = mn;
+    l = l * fo + pl * fn;
+    v = make_float4(v.x * fo + o.x * fn, v.y * fo + o.y * fn, v.z * fo + o.z * fn, v.w * fo + o.w * fn);
+  };
+  if (warp == 0) {
+    SlotInfo at{-1, 0, 0, 0};
+    if (lane < 2 * kWarps) at = info[lane];
+    const uint32_t valid = __ballot_sync(0xffffffffu, at.line >= 0);
+    const uint32_t below = valid & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, at.line, below != 0u ? 31 - __clz(below) : 0);
+    const bool start = at.line >= 0 && (below == 0u || prev != at.line);
+    const uint32_t starts = __ballot_sync(0xffffffffu, start);
+    const uint32_t later = starts & ~((2u << lane) - 1u);
+    if (lane < 2) ends[lane] = -1;
+    __syncwarp();
+    if (start) {
+      runs[__popc(starts & ((1u << lane) - 1u))] =
+          valid & ~((1u << lane) - 1u) & (later != 0u ? (later & -later) - 1u : ~0u);
+      if (at.line < c0 || at.line + at.tiles > c1) ends[at.line <= c0 ? 0 : 1] = lane;
+    }
+    if (lane == 0) *n_runs = __popc(starts);
+  }
+  __syncthreads();
+  const int work = *n_runs * units;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < work; i += kThreads) {
+    const int run = i / units, e = i - run * units;
+    uint32_t mask = runs[run];
+    const SlotInfo at = info[__ffs(mask) - 1];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (; mask != 0u; mask &= mask - 1u) {
+      const int k = __ffs(mask) - 1;
+      const float* part = reinterpret_cast<const float*>(
+          gbase + ((k & 1) ? static_cast<uint32_t>(k >> 1) * kStages * 2 * L::kCodes : L::kHead + (k >> 1) * L::kSlot));
+      add_part(v, m, l, reinterpret_cast<const float4*>(part)[e], part[L::kRows * HD + e / kF4],
+               part[L::kRows * HD + L::kRows + e / kF4]);
+    }
+    if (at.line >= c0 && at.line + at.tiles <= c1) {
+      put(at, e, v, m, l);
+    } else {
+      float* mine = p.part + (2LL * blockIdx.x + (at.line <= c0 ? 0 : 1)) * kPart;  // a part per end of the share
+      reinterpret_cast<float4*>(mine)[e] = v;
+      if (e % kF4 == 0) {
+        mine[L::kRows * HD + e / kF4] = m;
+        mine[L::kRows * HD + L::kRows + e / kF4] = l;
       }
     }
-    if (s0 < 0) break;
-    const Place at = locate(line);
-    const bool inside = line >= c0 && line + at.tiles <= c1;
-    auto put = [&](int e, const float4& v, float inv) {
-      const int r = e / kF4;
-      const int tok = r / p.group;
-      const int head = at.h * p.group + r - tok * p.group;
-      *reinterpret_cast<uint2*>(p.o + at.b * p.o_batch + tok * p.o_tok + head * p.o_head + e % kF4 * 4) =
-          make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
-    };
-    // Joins parts k0..k1 (get(k): O', m', l of unit e) in order, eight loads at a time.
-    auto join = [&](int e, int k0, int k1, auto get, float4& v, float& m, float& l) {
-      m = -INFINITY;
-      l = 0.f;
-      v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = k0; k <= k1; k += 8) {
+  }
+  if (ends[0] < 0 && ends[1] < 0) return;
+  // Count in; the CTA of a line's last part joins them all, in CTA order.
+  auto owner = [&](int u) {  // the CTA whose share holds tile u
+    const int big = more * (each + 1);
+    return u < big ? u / (each + 1) : more + (u - big) / each;
+  };
+  __syncthreads();  // the counting threads' releases cover the CTA's stores
+  if (threadIdx.x < 2) {
+    int parts = 0;  // of the line, if this CTA has to join them
+    if (ends[threadIdx.x] >= 0) {
+      const SlotInfo at = info[ends[threadIdx.x]];
+      const int n = owner(at.line + at.tiles - 1) - owner(at.line) + 1;
+      unsigned* count = p.count + static_cast<long long>(at.b) * p.kv_heads + at.h;
+      unsigned was;
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(was) : "l"(count) : "memory");
+      if (static_cast<int>(was) == n - 1) {
+        *count = 0u;  // ready for the next launch
+        parts = n;
+      }
+    }
+    runs[threadIdx.x] = static_cast<uint32_t>(parts);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int end = 0; end < 2; ++end) {
+    const int parts = static_cast<int>(runs[end]);
+    if (parts == 0) continue;
+    const SlotInfo at = info[ends[end]];
+    const int first = owner(at.line);
+    const float* part0 = p.part + 2LL * first * kPart;
+    // Only the first part may lie behind its CTA's first tile.
+    const int skip = at.line <= cta_begin(first) ? 0 : kPart;
+#pragma unroll 1
+    for (int e = threadIdx.x; e < units; e += kThreads) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int k = 0; k < parts; k += 8) {
         float4 o[8];
         float pm[8], pl[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          pm[i] = -INFINITY;
-          pl[i] = 0.f;
-          o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (k + i <= k1) get(k + i, e, o[i], pm[i], pl[i]);
+          const float* s = part0 + 2LL * min(k + i, parts - 1) * kPart + (k + i == 0 ? skip : 0);
+          pm[i] = k + i < parts ? __ldcg(s + L::kRows * HD + e / kF4) : -INFINITY;
+          pl[i] = k + i < parts ? __ldcg(s + L::kRows * HD + L::kRows + e / kF4) : 0.f;
+          o[i] = __ldcg(reinterpret_cast<const float4*>(s) + e);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float mn = fmaxf(m, pm[i]);
-          const float fo = m == mn ? 1.f : ex2_approx(m - mn);
-          const float fn = pm[i] == mn ? 1.f : ex2_approx(pm[i] - mn);
-          m = mn;
-          l = l * fo + pl[i] * fn;
-          v = make_float4(v.x * fo + o[i].x * fn, v.y * fo + o[i].y * fn, v.z * fo + o[i].z * fn, v.w * fo + o[i].w * fn);
-        }
+        for (int i = 0; i < 8; ++i)
+          if (k + i < parts) add_part(v, m, l, o[i], pm[i], pl[i]);
       }
-    };
-    auto in_shared = [&](int k, int e, float4& o, float& pm, float& pl) {
-      if (info[k] != line) return;
-      const float* s = reinterpret_cast<const float*>(
-          gbase + ((k & 1) ? static_cast<uint32_t>(k >> 1) * kStages * 2 * L::kCodes : L::kHead + (k >> 1) * L::kSlot));
-      pm = s[L::kRows * HD + e / kF4];
-      pl = s[L::kRows * HD + L::kRows + e / kF4];
-      o = reinterpret_cast<const float4*>(s)[e];
-    };
-    constexpr int kPart = L::kSlot / 4;
-    float* mine = p.part + (2LL * blockIdx.x + (line <= c0 ? 0 : 1)) * kPart;  // one part per end of the CTA's share
-    for (int e = lane; e < p.rows * kF4; e += 32) {
-      float4 v;
-      float m, l;
-      join(e, s0, s1, in_shared, v, m, l);
-      if (inside) {
-        put(e, v, inverse(m, l));
-      } else {
-        reinterpret_cast<float4*>(mine)[e] = v;
-        if (e % kF4 == 0) {
-          mine[L::kRows * HD + e / kF4] = m;
-          mine[L::kRows * HD + L::kRows + e / kF4] = l;
-        }
-      }
-    }
-    if (inside) continue;
-    // Count in; the last part of the line joins them all, in CTA order.
-    auto owner = [&](int u) {  // the CTA whose share holds tile u
-      const int big = more * (each + 1);
-      return u < big ? u / (each + 1) : more + (u - big) / each;
-    };
-    const int first = owner(line), last = owner(line + at.tiles - 1);
-    __threadfence();
-    __syncwarp();
-    unsigned n = 0;
-    unsigned* count = p.count + static_cast<long long>(at.b) * p.kv_heads + at.h;
-    if (lane == 0) {
-      n = atomicAdd(count, 1u) + 1u;
-      if (n == static_cast<unsigned>(last - first + 1)) *count = 0u;  // ready for the next launch
-    }
-    n = __shfl_sync(0xffffffffu, n, 0);
-    if (n != static_cast<unsigned>(last - first + 1)) continue;
-    __threadfence();
-    // Only the first part may lie behind its CTA's first tile.
-    const int first_slot = line <= cta_begin(first) ? 0 : 1;
-    auto in_global = [&](int k, int e, float4& o, float& pm, float& pl) {
-      const float* s = p.part + (2LL * k + (k == first ? first_slot : 0)) * kPart;
-      pm = __ldcg(s + L::kRows * HD + e / kF4);
-      pl = __ldcg(s + L::kRows * HD + L::kRows + e / kF4);
-      o = __ldcg(reinterpret_cast<const float4*>(s) + e);
-    };
-    for (int e = lane; e < p.rows * kF4; e += 32) {
-      float4 v;
-      float m, l;
-      join(e, first, last, in_global, v, m, l);
-      put(e, v, inverse(m, l));
+      put(at, e, v, m, l);
     }
   }
 }
