@@ -245,6 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_v);
     tma_prefetch_desc(&tm_o);
   }
+  pdl_start();
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -676,6 +678,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A thread takes 8 output values of a row; consecutive threads take consecutive rows.
 template <int HD>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
+  pdl_start();
+  pdl_wait();
   const int t = threadIdx.x;
   const int d8 = blockIdx.x % (HD / 8);
   int w = blockIdx.x / (HD / 8);  // (sequence, line, pair, tile)
@@ -722,13 +726,9 @@ cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
-  kernel<<<grid, kThreads, Smem<HD>::kBytes, stream>>>(tq, tk, tv, to, p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && p.n_split > 1) {
-    const int blocks = p.batch * p.lines * p.pairs * 2 * (HD / 8);
-    kv8_join_kernel<HD><<<blocks, 128, 0, stream>>>(p);
-    e = cudaGetLastError();
-  }
+  cudaError_t e = launch_pdl(kernel, grid, kThreads, Smem<HD>::kBytes, stream, tq, tk, tv, to, p);
+  if (e == cudaSuccess && p.n_split > 1)
+    e = launch_pdl(kv8_join_kernel<HD>, p.batch * p.lines * p.pairs * 2 * (HD / 8), 128, 0, stream, p);
   return e;
 }
 

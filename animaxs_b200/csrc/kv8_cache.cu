@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
   constexpr int kRowsPerPass = kWriteThreads / kLanes;
   constexpr int kPasses = kKv8Block / kRowsPerPass;
   __shared__ float warp_max[kWriteThreads / 32];
+  pdl_start();
   int w = blockIdx.x;
   const int kv = w & 1;
   w >>= 1;
@@ -50,6 +51,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
   w /= p.kv_heads;
   const int b = w / window;
   const int wi = w % window;
+  pdl_wait();
   const long long start = p.starts != nullptr ? p.starts[b] : p.start;
   const int n = p.counts != nullptr ? min(max(p.counts[b], 0), p.tokens) : p.tokens;
   const long long first = start > 0 ? start : 0;                               // first written position
@@ -128,6 +130,7 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadPar
   constexpr int kLanes = HD / 8;
   constexpr int kRowsPerPass = kReadThreads / kLanes;
   constexpr int kPasses = kKv8Block / kRowsPerPass;
+  pdl_start();
   int w = blockIdx.x;
   const int kv = w & 1;
   w >>= 1;
@@ -135,6 +138,7 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadPar
   w /= p.kv_heads;
   const int b = w / chunks;
   const int t0 = w % chunks * kKv8Block;
+  pdl_wait();
   const int len = p.lens != nullptr ? p.lens[b] : p.capacity;
   const int lane = threadIdx.x % kLanes;
   const long long bh = static_cast<long long>(b) * p.kv_heads + h;
@@ -187,8 +191,7 @@ cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream) {
   auto kernel = p.format == kKv8Int8
                     ? (p.head_dim == 128 ? kv8_write_kernel<kKv8Int8, 128> : kv8_write_kernel<kKv8Int8, 64>)
                     : (p.head_dim == 128 ? kv8_write_kernel<kKv8E4m3, 128> : kv8_write_kernel<kKv8E4m3, 64>);
-  kernel<<<static_cast<unsigned>(ctas), kWriteThreads, 0, stream>>>(p, window);
-  return cudaGetLastError();
+  return launch_pdl(kernel, static_cast<unsigned>(ctas), kWriteThreads, 0, stream, p, window);
 }
 
 cudaError_t launch_kv8_read(const Kv8ReadParams& p, cudaStream_t stream) {
@@ -198,8 +201,7 @@ cudaError_t launch_kv8_read(const Kv8ReadParams& p, cudaStream_t stream) {
   auto kernel = p.format == kKv8Int8
                     ? (p.head_dim == 128 ? kv8_read_kernel<kKv8Int8, 128> : kv8_read_kernel<kKv8Int8, 64>)
                     : (p.head_dim == 128 ? kv8_read_kernel<kKv8E4m3, 128> : kv8_read_kernel<kKv8E4m3, 64>);
-  kernel<<<static_cast<unsigned>(ctas), kReadThreads, 0, stream>>>(p, chunks);
-  return cudaGetLastError();
+  return launch_pdl(kernel, static_cast<unsigned>(ctas), kReadThreads, 0, stream, p, chunks);
 }
 
 }  // namespace ax

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "../../include/animaxs_attn.h"
 
@@ -65,6 +66,31 @@ __device__ __forceinline__ uint32_t kv8_pack4(float a, float b, float c, float d
         : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
   }
+}
+
+// Programmatic dependent launch: the kernels of the cache follow one another
+// (a step writes, then attends), so each may be set up while the one before it
+// ends.  pdl_wait() returns when that one has completed and its writes are
+// visible; nothing of global memory is touched before it.
+__device__ __forceinline__ void pdl_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+                       Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 // A sequence's length, within [0, kv_len].

@@ -122,12 +122,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = base + warp * kStages * 2 * L::kCodes;
   const uint32_t bar = base + L::kBar + warp * kStages * 8;
 
-  // prefix[t]: tiles of one line of the sequences before group t (kThreads
-  // groups of `per` sequences).
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  auto tiles_in = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
-  int scan = 0;
-  for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) scan += tiles_in(b);
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
     info[2 * warp].line = info[2 * warp + 1].line = -1;
@@ -139,6 +133,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  pdl_start();
+  pdl_wait();
+  // prefix[t]: tiles of one line of the sequences before group t (kThreads
+  // groups of `per` sequences).
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  auto tiles_in = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
+  int scan = 0;
+  for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) scan += tiles_in(b);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, scan, o);
@@ -587,6 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     runs[threadIdx.x] = static_cast<uint32_t>(parts);
   }
   __syncthreads();
+  float4* sums = reinterpret_cast<float4*>(gbase);  // [kThreads] O', then (m', l); the rings are idle
 #pragma unroll 1
   for (int end = 0; end < 2; ++end) {
     const int parts = static_cast<int>(runs[end]);
@@ -596,26 +599,50 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float* part0 = p.part + 2LL * first * kPart;
     // Only the first part may lie behind its CTA's first tile.
     const int skip = at.line <= cta_begin(first) ? 0 : kPart;
+    // More than eight parts: groups of threads take a range of them each (one
+    // token on 131071 keys 55.6 -> 53.8 us); up to eight are one round of loads.
+    const int groups = parts > 8 ? max(kThreads / units, 1) : 1;
+    const int group = static_cast<int>(threadIdx.x) / units;
+    if (groups > 1) __syncthreads();  // sums is free
 #pragma unroll 1
-    for (int e = threadIdx.x; e < units; e += kThreads) {
+    for (int e = threadIdx.x - group * units; group < groups && e < units; e += kThreads) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       float m = -INFINITY, l = 0.f;
+      const int k1 = parts * (group + 1) / groups;
 #pragma unroll 1
-      for (int k = 0; k < parts; k += 8) {
+      for (int k = parts * group / groups; k < k1; k += 8) {
         float4 o[8];
         float pm[8], pl[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float* s = part0 + 2LL * min(k + i, parts - 1) * kPart + (k + i == 0 ? skip : 0);
-          pm[i] = k + i < parts ? __ldcg(s + L::kRows * HD + e / kF4) : -INFINITY;
-          pl[i] = k + i < parts ? __ldcg(s + L::kRows * HD + L::kRows + e / kF4) : 0.f;
+          const int x = min(k + i, k1 - 1);
+          const float* s = part0 + 2LL * x * kPart + (x == 0 ? skip : 0);
+          pm[i] = __ldcg(s + L::kRows * HD + e / kF4);
+          pl[i] = __ldcg(s + L::kRows * HD + L::kRows + e / kF4);
           o[i] = __ldcg(reinterpret_cast<const float4*>(s) + e);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (k + i < parts) add_part(v, m, l, o[i], pm[i], pl[i]);
+          if (k + i < k1) add_part(v, m, l, o[i], pm[i], pl[i]);
       }
-      put(at, e, v, m, l);
+      if (groups == 1) {
+        put(at, e, v, m, l);
+      } else {
+        sums[threadIdx.x] = v;
+        reinterpret_cast<float2*>(sums + kThreads)[threadIdx.x] = make_float2(m, l);
+      }
+    }
+    if (groups == 1) continue;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < units) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < groups; ++i) {
+        const float2 ml = reinterpret_cast<const float2*>(sums + kThreads)[i * units + threadIdx.x];
+        add_part(v, m, l, sums[i * units + threadIdx.x], ml.x, ml.y);
+      }
+      put(at, threadIdx.x, v, m, l);
     }
   }
 }
@@ -632,8 +659,7 @@ cudaError_t launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8Att
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
-  kernel<<<grid, kThreads, RowsSmem<HD, NT>::kBytes, stream>>>(tk, tv, p);
-  return cudaGetLastError();
+  return launch_pdl(kernel, grid, kThreads, RowsSmem<HD, NT>::kBytes, stream, tk, tv, p);
 }
 template <int FMT, int HD>
 cudaError_t launch_hd(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
