@@ -6,31 +6,46 @@
 // one dependent chain (positions -> rows -> maximum -> codes) when there is not.
 #include "kernels.h"
 #include "kv8_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ax {
 namespace {
 
 constexpr int kWriteThreads = 128;
 
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
 // The magnitudes of a pair, 0 in place of what is not finite.
 __device__ __forceinline__ __half2 finite_abs(uint32_t w) {
-  const __half2 a = __habs2(*reinterpret_cast<const __half2*>(&w));
+  const __half2 a = __habs2(as_half2(w));
   const __half2 inf = __halves2half2(__ushort_as_half(0x7C00), __ushort_as_half(0x7C00));
-  const uint32_t m = __hlt2_mask(a, inf) & *reinterpret_cast<const uint32_t*>(&a);  // NaN compares false
-  return *reinterpret_cast<const __half2*>(&m);
+  return as_half2(__hlt2_mask(a, inf) & as_u32(a));  // NaN compares false
 }
 // A pair with 0 in place of NaN.
-__device__ __forceinline__ uint32_t nan_to_zero(uint32_t w) {
-  const __half2 h = *reinterpret_cast<const __half2*>(&w);
-  return __heq2_mask(h, h) & w;
-}
-template <int FMT>
+__device__ __forceinline__ uint32_t nan_to_zero(uint32_t w) { return __heq2_mask(as_half2(w), as_half2(w)) & w; }
+
+// Four values to codes.  kFinite: all of them are finite, so that none is
+// beyond +-M after the scaling (a * (1 / (a / M)) rounds to M) and none is NaN.
+template <int FMT, bool kFinite>
 __device__ __forceinline__ uint32_t quantise4(uint32_t a, uint32_t b, float inv) {
-  a = nan_to_zero(a);
-  b = nan_to_zero(b);
-  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
-  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  return kv8_pack4<FMT>(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
+  if constexpr (!kFinite) {
+    a = nan_to_zero(a);
+    b = nan_to_zero(b);
+  }
+  float2 x = __half22float2(as_half2(a)), y = __half22float2(as_half2(b));
+  // The product is rounded before it is rounded to an integer: a packed
+  // multiply would be contracted with the packed addition below, .rn or not.
+  x = make_float2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
+  y = make_float2(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
+  if constexpr (FMT == kKv8Int8 && kFinite) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low mantissa bits are the rounded integer
+    const float2 k2 = make_float2(kMagic, kMagic), p = add2(x, k2), q = add2(y, k2);
+    return prmt(prmt(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040u),
+                prmt(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040u), 0x5410u);
+  } else {
+    return kv8_pack4<FMT>(x.x, x.y, y.x, y.y);
+  }
 }
 
 // One CTA per (64-token block, head, sequence, K or V): it alone reads and
@@ -74,13 +89,30 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
     const int r = row0 + i * kRowsPerPass;
     if (r >= lo && r < hi) x[i] = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
   }
-  __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+  // Largest magnitude; NaN and infinity show in it and send the thread to the
+  // slower form (most of the kernel's instructions are per value, and it is
+  // bound by them: 512 tokens x 16 heads x 8 prompts 13.0 us with the checks
+  // on every value).
+  const __half2 none = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+  __half2 mx = none;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = row0 + i * kRowsPerPass;
     if (r >= lo && r < hi)
-      mx = __hmax2(mx, __hmax2(__hmax2(finite_abs(x[i].x), finite_abs(x[i].y)),
-                               __hmax2(finite_abs(x[i].z), finite_abs(x[i].w))));
+      mx = __hmax2_nan(mx, __hmax2_nan(__hmax2_nan(__habs2(as_half2(x[i].x)), __habs2(as_half2(x[i].y))),
+                                       __hmax2_nan(__habs2(as_half2(x[i].z)), __habs2(as_half2(x[i].w)))));
+  }
+  const bool finite = __hlt(__low2half(mx), __ushort_as_half(0x7C00)) && __hlt(__high2half(mx), __ushort_as_half(0x7C00));
+  if (!finite) {
+    mx = none;
+#pragma unroll 1
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = row0 + i * kRowsPerPass;
+      if (r >= lo && r < hi) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+        mx = __hmax2(mx, __hmax2(__hmax2(finite_abs(v.x), finite_abs(v.y)), __hmax2(finite_abs(v.z), finite_abs(v.w))));
+      }
+    }
   }
   float a = fmaxf(__low2float(mx), __high2float(mx));
 #pragma unroll
@@ -91,13 +123,25 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
   for (int i = 0; i < kWriteThreads / 32; ++i) a = fmaxf(a, warp_max[i]);
   const float s = fmaxf(__fmul_rn(a, 1.f / kKv8Top<FMT>), before);
   const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+  if (finite) {
+    // With a scale of 0 every finite value is 0, and 0 * 0 rounds to code 0.
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = row0 + i * kRowsPerPass;
-    if (r >= lo && r < hi) {
-      uint2 c = make_uint2(0u, 0u);
-      if (inv > 0.f) c = make_uint2(quantise4<FMT>(x[i].x, x[i].y, inv), quantise4<FMT>(x[i].z, x[i].w, inv));
-      *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD) = c;
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = row0 + i * kRowsPerPass;
+      if (r >= lo && r < hi)
+        *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD) =
+            make_uint2(quantise4<FMT, true>(x[i].x, x[i].y, inv), quantise4<FMT, true>(x[i].z, x[i].w, inv));
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = row0 + i * kRowsPerPass;
+      if (r >= lo && r < hi) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+        uint2 c = make_uint2(0u, 0u);
+        if (inv > 0.f) c = make_uint2(quantise4<FMT, false>(v.x, v.y, inv), quantise4<FMT, false>(v.z, v.w, inv));
+        *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD) = c;
+      }
     }
   }
   if (threadIdx.x == 0) *scale = s;
