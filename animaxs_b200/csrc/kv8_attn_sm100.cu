@@ -443,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int run = part * (HD / 32) + i;
           c[i] = ld_shared_v4u(src + (HD == 128 ? run ^ (key & 7) : run ^ ((key >> 1) & 3)) * 16);
         }
+        // The slot's next tensor copy must not overtake these reads.
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(kBarRawEmpty + slot));
         // What lies past the length may decode to NaN: such keys become zeros.

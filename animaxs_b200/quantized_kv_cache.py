@@ -53,7 +53,8 @@ class QuantizedKVCache:
         dtype = torch.int8 if format == "int8" else torch.float8_e4m3fn
         codes = [torch.empty((batch, kv_heads, capacity, head_dim), dtype=dtype, device=dev) for _ in range(2)]
         blocks = scale_bytes.value // 4 // (batch * kv_heads)
-        scales = [torch.empty((batch, kv_heads, blocks), dtype=torch.float32, device=dev) for _ in range(2)]
+        # Zeros, so that a write that starts inside a block nothing was written to finds no scale there.
+        scales = [torch.zeros((batch, kv_heads, blocks), dtype=torch.float32, device=dev) for _ in range(2)]
         self._bind(executor, *codes, *scales)
 
     @classmethod

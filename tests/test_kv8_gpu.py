@@ -308,6 +308,51 @@ def test_attention_is_repeatable_and_uses_its_stream(ex, q_len, kv_len):
     assert torch.equal(wide[..., 128:], first) and (wide[..., :128] == 3).all()
 
 
+@pytest.mark.parametrize("batch,q_len,heads,kv_heads,dim,kv_len,causal", [
+    (2, 1700, 16, 8, 64, 378, False), (1, 600, 16, 16, 128, 2000, False), (3, 294, 16, 8, 64, 648, True),
+    (20, 1, 16, 8, 128, 1500, True), (4, 8, 4, 2, 64, 2000, False)])
+def test_attention_many_calls_agree(ex, batch, q_len, heads, kv_heads, dim, kv_len, causal):
+    """Bit for bit over 400 calls: a copy that overtook the readers of its shared-memory slot would show here."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(4)
+    cache = _cache(ex, "e4m3", batch, kv_len, kv_heads, dim)
+    k, v = (torch.randn((batch, kv_len, kv_heads, dim), generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn((batch, q_len, heads, dim), generator=g, device="cuda").half()
+    cache.write(k, v)
+    outs = [cache.attention(q, causal=causal) for _ in range(2)]
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(400):
+        cache.attention(q, outs[1], causal=causal)
+        differ += (outs[1].view(torch.int16) != outs[0].view(torch.int16)).any()
+    assert int(differ) == 0
+
+
+def test_positions_past_32_bits(ex):
+    """Codes beyond 4 GiB of a buffer: the third sequence of three of 18 million tokens, and its last block."""
+    import torch
+    g = np.random.default_rng(6)
+    cap = 18_000_000
+    cache = _cache(ex, "int8", 3, cap, 1, 128, garbage=False)
+    k, v = (_rand(g, (3, 300, 1, 128)) for _ in range(2))
+    cache.write(_dev(k), _dev(v))
+    q = _rand(g, (3, 4, 2, 128))
+    lens = [0, 17, 300]
+    many = _rand(g, (3, 70, 2, 128))
+    for queries in (q, many):
+        out = cache.attention(_dev(queries), lens=_ints(lens), causal=True)
+        kd = ora.decode(_values(cache.k_codes[:, :, :300]), cache.k_scale[:, :, :5].cpu().numpy())
+        vd = ora.decode(_values(cache.v_codes[:, :, :300]), cache.v_scale[:, :, :5].cpu().numpy())
+        ref = ora.attention(queries, kd, vd, lens, True)
+        bound = 2.0 ** -10 * np.abs(ref) + (2.0 ** -10 + 300 * 2.0 ** -25) * np.abs(vd).max()
+        _assert_close(out.double().cpu().numpy(), ref, bound)
+    cache.write(_dev(k), _dev(v), cap - 300)
+    rk, rv = cache.read(cap - 300, 300)
+    for got, x in ((rk, k), (rv, v)):
+        err = np.abs(got.double().cpu().numpy() - x.astype(np.float64))
+        assert (err <= np.abs(x).max() / 127 * 0.51 + np.abs(x) * 2.0 ** -10).all()
+    assert torch.equal(cache.read(cap - 1, 1)[0], rk[:, -1:])
+
+
 def test_attention_normalises_q(ex):
     """qk_norm="rms" is the attention prologue's normalisation followed by the plain call."""
     import torch
