@@ -51,9 +51,12 @@ class QuantizedKVCache:
         raise_for(rc, "invalid 8-bit K/V cache shape (head_dim 64 or 128, positive sizes)")
         dev = torch.device("cuda", executor.device)
         dtype = torch.int8 if format == "int8" else torch.float8_e4m3fn
-        codes = [torch.empty((batch, kv_heads, capacity, head_dim), dtype=dtype, device=dev) for _ in range(2)]
+        # Zeros: a key that a causal mask hides still meets a weight of 0, which a NaN code (e4m3 has them) would turn
+        # into NaN where ``lens`` counts positions not written yet, as a padded batch of prompts does; and a write
+        # that starts inside a block nothing was written to finds no scale there.
+        codes = [torch.zeros((batch, kv_heads, capacity, head_dim), dtype=torch.int8, device=dev).view(dtype)
+                 for _ in range(2)]
         blocks = scale_bytes.value // 4 // (batch * kv_heads)
-        # Zeros, so that a write that starts inside a block nothing was written to finds no scale there.
         scales = [torch.zeros((batch, kv_heads, blocks), dtype=torch.float32, device=dev) for _ in range(2)]
         self._bind(executor, *codes, *scales)
 
