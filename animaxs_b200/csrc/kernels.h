@@ -184,6 +184,10 @@ struct Kv8AttnParams {
   const float* k_scale;
   const float* v_scale;
   int rows;             // group * q_len: query rows of a kv head
+  // Few rows (kv8_rows_plan): each line to a cluster of its own, of 2^cluster_log2
+  // CTAs; floor(65536 / group) + 1, which divides the row numbers.
+  bool alone;
+  int cluster_log2, group_inv;
   float* part;          // workspace: partial results (kv8_rows_part_floats, kv8_attn_part_floats)
   unsigned int* count;  // arrivals per (sequence, kv head), zero between launches
   unsigned int* status;
@@ -195,7 +199,7 @@ struct Kv8AttnParams {
 // Attention of up to 16 query rows over the cache (kv8_rows_sm100.cu); tk/tv are
 // ax_make_tmap_codes maps with boxes of kv8_rows_tile() rows.
 int kv8_rows_tile();
-int kv8_rows_grid(const Kv8AttnParams& p, int sms);
+int kv8_rows_plan(Kv8AttnParams* p, int sms);
 size_t kv8_rows_part_floats(int head_dim, int grid);
 cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid,
                             int dev, cudaStream_t stream);

@@ -328,7 +328,7 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   if (rc != ANIMAXS_OK) return rc;
   cudaError_t e;
   if (few) {
-    const int grid = ax::kv8_rows_grid(p, ctx->num_sms);
+    const int grid = ax::kv8_rows_plan(&p, ctx->num_sms);
     rc = ensure_split(ctx, ax::kv8_rows_part_floats(d->head_dim, grid), static_cast<size_t>(heads));
     if (rc != ANIMAXS_OK) return rc;
     p.part = ctx->kv8_part;

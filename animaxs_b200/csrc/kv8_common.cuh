@@ -78,19 +78,27 @@ __device__ __forceinline__ void pdl_start() {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
-                       Args&&... args) {
+cudaError_t launch_pdl_cluster(void (*kernel)(Params...), unsigned grid, unsigned cluster, unsigned threads,
+                               size_t smem, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+                       Args&&... args) {
+  return launch_pdl_cluster(kernel, grid, 1, threads, smem, stream, std::forward<Args>(args)...);
 }
 
 // A sequence's length, within [0, kv_len].

@@ -14,15 +14,25 @@
 // anyway, p' never exceeds 2^8 (see the lazy rescale below) whatever the
 // scales, and the codes enter both products unscaled, exact as fp16.
 //
-// Work: every (sequence, kv head) is a line of 32-key tiles; all lines together
-// are cut into equal contiguous shares, one per warp (eight warps per SM), so
-// ragged lengths and single long sequences load the SMs alike.  A warp runs by
-// itself: its lane 0 keeps a ring of tiles in flight by TMA, all lanes take a
-// tile into registers, and no other warp is waited for until the share is done.
-// Then the CTA's warps join the parts of lines that cross a warp's share, and
-// what crosses the CTA's goes through a workspace: each CTA stores its part
-// (m', l, O') and counts itself in, and the last one to arrive joins the
-// parts in CTA order, so the result does not depend on the order of arrival.
+// Work: every (sequence, kv head) is a line of 32-key tiles.  A warp takes a
+// contiguous share of them and runs by itself: its lane 0 keeps a ring of tiles
+// in flight by TMA, all lanes take a tile into registers, and no other warp is
+// waited for until the share is done.  Shares are cut in one of two ways:
+//  * a cluster of 1 to 8 CTAs to each line, where that leaves a warp few tiles.
+//    The warps of a CTA join their parts in shared memory, the CTAs of the
+//    cluster theirs in distributed shared memory;
+//  * equal shares of all lines together, so that ragged lengths and single long
+//    sequences load the SMs alike.  What crosses a CTA's share goes through a
+//    workspace: each CTA stores its part (m', l, O') and counts itself in, and
+//    the last one to arrive joins the parts.
+// Parts are joined in warp and CTA order, so the result does not depend on the
+// order of arrival.
+//
+// Measured (int8, group 2, head_dim 128; GPU time of a call in a graph): batch
+// 1 x 8 kv heads, one query token on 300 keys 4.9 us (equal shares 8.0, of which
+// 3 are the join through global memory), on 2048 keys 5.4 (8.5); a tile costs a
+// warp 1.4 us when nothing is in flight before it, hence the bound on a
+// cluster's shares.
 //
 // Products: m16n8k16 mma.sync with the cache as the 16-wide operand and the
 // query rows as the 8-wide one (one or two column tiles):
@@ -45,6 +55,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileKeys = 32;
+constexpr int kAlone = 3;          // tiles of a warp up to which a line has a cluster of its own (kv8_rows_plan)
 constexpr float kRescale = 8.f;    // log2 units by which the maximum may lag
 constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
@@ -88,6 +99,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 __device__ __forceinline__ uint2 ld_shared_v2u(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_v4f(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2f(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
@@ -135,39 +159,71 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   pdl_start();
   pdl_wait();
+  const int lines = p.batch * p.kv_heads;
+  int c0 = 0, c1 = 0;  // the CTA's tiles
+  bool alone = p.alone;  // a cluster to each line, known before the lengths are
+  const int rank = static_cast<int>(blockIdx.x) & ((1 << p.cluster_log2) - 1);  // in the cluster
   // prefix[t]: tiles of one line of the sequences before group t (kThreads
   // groups of `per` sequences).
   const int per = (p.batch + kThreads - 1) / kThreads;
   auto tiles_in = [&](int b) { return (kv8_len(p.lens, p.kv_valid, p.kv_len, b) + kTileKeys - 1) / kTileKeys; };
-  int scan = 0;
-  for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) scan += tiles_in(b);
+  int all = 0, longest = 0;
+  if (!alone) {
+    int scan = 0;
+    for (int b = threadIdx.x * per; b < min((static_cast<int>(threadIdx.x) + 1) * per, p.batch); ++b) {
+      const int n = tiles_in(b);
+      scan += n;
+      longest = max(longest, n);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += u;
-  }
-  int* warp_sum = reinterpret_cast<int*>(gbase + L::kHead);  // free until a share ends
-  if (lane == 31) warp_sum[warp] = scan;
-  __syncthreads();
-  int before = 0, all = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += u;
+    }
+    int* warp_sum = reinterpret_cast<int*>(gbase + L::kHead);  // free until a share ends
+    if (lane == 31) {
+      warp_sum[warp] = scan;
+      warp_sum[kWarps + warp] = longest;
+    }
+    __syncthreads();
+    int before = 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    const int v = warp_sum[i];
-    if (i < warp) before += v;
-    all += v;
+    for (int i = 0; i < kWarps; ++i) {
+      const int v = warp_sum[i];
+      if (i < warp) before += v;
+      all += v;
+      longest = max(longest, warp_sum[kWarps + i]);
+    }
+    prefix[threadIdx.x + 1] = scan + before;
   }
-  prefix[threadIdx.x + 1] = scan + before;
   __syncthreads();
   // Up to kThreads sequences their tiles are in shared memory.
   auto tiles_of = [&](int b) { return per == 1 ? prefix[b + 1] - prefix[b] : tiles_in(b); };
-  const int total = all * p.kv_heads;  // a cache of 2^46 codes has fewer than 2^31 tiles on any GPU
   // Shares: no more CTAs than tiles, so that every CTA has one and arrives
   // where it is counted.  The first `more` CTAs take one tile more.
-  const int grid = max(min(static_cast<int>(gridDim.x), total), 1);
-  const int each = total / grid, more = total - each * grid;
+  int grid = 1, each = 0, more = 0;
+  if (!alone) {
+    const int total = all * p.kv_heads;  // a cache of 2^46 codes has fewer than 2^31 tiles on any GPU
+    grid = max(min(static_cast<int>(gridDim.x), total), 1);
+    each = total / grid;
+    more = total - each * grid;
+    // Or known only now: a CTA to each line when no line is long.
+    alone = lines <= static_cast<int>(gridDim.x) && longest <= kWarps * kAlone + each;
+  }
   auto cta_begin = [&](int i) { return i * each + min(i, more); };
-  const bool idle = static_cast<int>(blockIdx.x) >= grid;
-  const int c0 = idle ? total : cta_begin(blockIdx.x), c1 = idle ? total : cta_begin(blockIdx.x + 1);
+  Place mine{0, 0, 0, 0};
+  if (alone) {
+    const int line = static_cast<int>(blockIdx.x) >> p.cluster_log2;
+    mine.b = line / p.kv_heads;
+    mine.h = line - mine.b * p.kv_heads;
+    if (mine.b < p.batch) mine.tiles = tiles_in(mine.b);
+    c0 = (mine.tiles * rank) >> p.cluster_log2;
+    c1 = (mine.tiles * (rank + 1)) >> p.cluster_log2;
+  } else if (static_cast<int>(blockIdx.x) < grid) {
+    c0 = cta_begin(blockIdx.x);
+    c1 = cta_begin(blockIdx.x + 1);
+  }
   const int u0 = c0 + (c1 - c0) * warp / kWarps, u1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
   static_assert(kThreads == 256, "locate() searches 32 x 8 groups");
   auto locate = [&](int u) {  // by a converged warp
@@ -196,8 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       at.tiles = tiles_of(++at.b);
     } while (at.tiles == 0);
   };
+  auto row_token = [&](int r) { return (r * p.group_inv) >> 16; };  // r / group
   auto store8 = [&](int b, int h, int row, int d, const float (&v)[8], float inv) {  // 8 outputs of a row
-    const int tok = row / p.group;
+    const int tok = row_token(row);
     const int head = h * p.group + row - tok * p.group;
     *reinterpret_cast<uint4*>(p.o + b * p.o_batch + tok * p.o_tok + head * p.o_head + d) =
         make_uint4(pack_half2(v[0] * inv, v[1] * inv), pack_half2(v[2] * inv, v[3] * inv),
@@ -206,12 +263,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   // A row without keys has m' = -inf and l = 0 and becomes 0; one with NaN scores has l = NaN.
   auto inverse = [](float m, float l) { return m == -INFINITY && l == l ? 0.f : 1.f / l; };
   // Rows of sequences without keys.
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (tiles_of(b) > 0) continue;
-    const float zero[8] = {};
-    for (int i = threadIdx.x; i < p.rows * p.kv_heads * (HD / 8); i += kThreads) {
-      const int r = i / (HD / 8);
-      store8(b, r / p.rows, r % p.rows, i % (HD / 8) * 8, zero, 0.f);
+  const float zero[8] = {};
+  if (alone) {
+    if (mine.tiles == 0 && mine.b < p.batch && rank == 0)
+      for (int i = threadIdx.x; i < p.rows * (HD / 8); i += kThreads)
+        store8(mine.b, mine.h, i / (HD / 8), i % (HD / 8) * 8, zero, 0.f);
+  } else {
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (tiles_of(b) > 0) continue;
+      for (int i = threadIdx.x; i < p.rows * p.kv_heads * (HD / 8); i += kThreads) {
+        const int r = i / (HD / 8);
+        store8(b, r / p.rows, r % p.rows, i % (HD / 8) * 8, zero, 0.f);
+      }
     }
   }
 
@@ -219,7 +282,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   if (u0 < u1) {
     // ------------------------------------------------------- the warp's share --
-    Place at = locate(u0);
+    Place at = mine;
+    if (alone)
+      at.tile = u0;
+    else
+      at = locate(u0);
     Place ahead = at;  // the next tile to load (lane 0)
     int ua = u0;
     auto load = [&](uint32_t st) {
@@ -256,13 +323,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int r = 8 * nt + 2 * c + x;
-          lim[nt][x] = p.causal && r < p.rows ? min(len, len - p.q_len + r / p.group + 1) : len;
+          lim[nt][x] = p.causal && r < p.rows ? min(len, len - p.q_len + row_token(r) + 1) : len;
         }
         const int r = 8 * nt + g;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) qf[nt][k][0] = qf[nt][k][1] = 0u;
         if (r < p.rows) {
-          const int tok = r / p.group;
+          const int tok = row_token(r);
           const int head = seg.h * p.group + r - tok * p.group;
           // This lane's k indexes: HD / 4 consecutive values of the row, four of them in each MMA step.
           const uint4* src = reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + tok * p.q_tok + head * p.q_head +
@@ -491,6 +558,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < kStages; ++i) mbar_wait_drain(bar + 8 * i, ph ^ (i < static_cast<int>(st) ? 1u : 0u));
   }
   __syncthreads();
+  const int units = p.rows * kF4;
+  if (alone) {
+    // --------------------------------------- the line's parts in this cluster --
+    if (mine.tiles < 2) return;  // no keys, or one warp had them all
+    const bool joint = p.cluster_log2 != 0;
+    if (!joint && (*abort_flag != 0 || info[2 * (kWarps - 1)].line < 0)) return;
+    auto put = [&](int e, const float4& v, float m, float l) {
+      const float inv = inverse(m, l);
+      const int r = e / kF4;
+      const int tok = row_token(r);
+      const int head = mine.h * p.group + r - tok * p.group;
+      *reinterpret_cast<uint2*>(p.o + mine.b * p.o_batch + tok * p.o_tok + head * p.o_head + e % kF4 * 4) =
+          make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+    };
+    // Sum of eight parts whose loads are all in flight; get(i, v, m, l) says whether there is an i-th.
+    auto join = [&](auto get, float4& v, float& m, float& l) {
+      float pm[8], pl[8];
+      float4 o[8];
+      m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pm[i] = -INFINITY;
+        pl[i] = 0.f;
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        get(i, o[i], pm[i], pl[i]);
+        m = fmaxf(m, pm[i]);
+      }
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = pm[i] == m ? 1.f : ex2_approx(pm[i] - m);
+        l = fmaf(pl[i], f, l);
+        v = make_float4(fmaf(o[i].x, f, v.x), fmaf(o[i].y, f, v.y), fmaf(o[i].z, f, v.z), fmaf(o[i].w, f, v.w));
+      }
+    };
+    float4 v;
+    float m, l;
+    float4* part_v = reinterpret_cast<float4*>(gbase);                      // the CTA's part: the rings are idle
+    float* part_ml = reinterpret_cast<float*>(gbase) + L::kRows * HD;       // (m', l) per row
+#pragma unroll 1
+    for (int e = threadIdx.x; e < units; e += kThreads) {
+      static_assert(kWarps == 8, "join() takes eight parts");
+      join([&](int i, float4& ov, float& om, float& ol) {
+        const float* part = reinterpret_cast<const float*>(gbase + L::kHead + i * L::kSlot);
+        if (info[2 * i].line >= 0) {
+          ov = reinterpret_cast<const float4*>(part)[e];
+          om = part[L::kRows * HD + e / kF4];
+          ol = part[L::kRows * HD + L::kRows + e / kF4];
+        }
+      }, v, m, l);
+      if (!joint) {
+        put(e, v, m, l);
+      } else {
+        part_v[e] = v;
+        if (e % kF4 == 0) reinterpret_cast<float2*>(part_ml)[e / kF4] = make_float2(m, l);
+      }
+    }
+    if (!joint) return;
+    __syncwarp();
+    cluster_sync();
+    // Each CTA of the cluster joins a share of the outputs, in CTA order.
+    const int n = 1 << p.cluster_log2;
+#pragma unroll 1
+    for (int e = rank + n * static_cast<int>(threadIdx.x); e < units; e += n * kThreads) {
+      const uint32_t at_v = base + e * 16u, at_ml = base + L::kRows * HD * 4u + e / kF4 * 8u;
+      join([&](int i, float4& ov, float& om, float& ol) {
+        if (i < n) {
+          ov = ld_cluster_v4f(mapa_shared(at_v, i));
+          const float2 ml = ld_cluster_v2f(mapa_shared(at_ml, i));
+          om = ml.x;
+          ol = ml.y;
+        }
+      }, v, m, l);
+      put(e, v, m, l);
+    }
+    __syncwarp();
+    cluster_sync();  // the parts have been read
+    return;
+  }
   if (*abort_flag != 0 || c0 >= c1) return;
 
   // ------------------------------------------- lines that cross warps or CTAs --
@@ -502,12 +649,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* runs = reinterpret_cast<uint32_t*>(prefix);          // [kWarps + 1]
   int* ends = prefix + kWarps + 2;                               // slot index of the line, -1: none
   volatile int* n_runs = prefix + kWarps + 4;
-  const int units = p.rows * kF4;
   constexpr int kPart = L::kSlot / 4;
   auto put = [&](const SlotInfo& at, int e, const float4& v, float m, float l) {
     const float inv = inverse(m, l);
     const int r = e / kF4;
-    const int tok = r / p.group;
+    const int tok = row_token(r);
     const int head = at.h * p.group + r - tok * p.group;
     *reinterpret_cast<uint2*>(p.o + at.b * p.o_batch + tok * p.o_tok + head * p.o_head + e % kF4 * 4) =
         make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
@@ -659,7 +805,7 @@ cudaError_t launch_nt(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8Att
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
-  return launch_pdl(kernel, grid, kThreads, RowsSmem<HD, NT>::kBytes, stream, tk, tv, p);
+  return launch_pdl_cluster(kernel, grid, 1u << p.cluster_log2, kThreads, RowsSmem<HD, NT>::kBytes, stream, tk, tv, p);
 }
 template <int FMT, int HD>
 cudaError_t launch_hd(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, int dev,
@@ -671,9 +817,21 @@ cudaError_t launch_hd(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8Att
 }  // namespace
 
 // One CTA per SM, but none without a tile when every sequence is as long as it can be.
-int kv8_rows_grid(const Kv8AttnParams& p, int sms) {
-  const long long tiles =
-      static_cast<long long>(p.batch) * p.kv_heads * ((p.kv_len + kTileKeys - 1) / kTileKeys);
+int kv8_rows_plan(Kv8AttnParams* p, int sms) {
+  const long long lines = static_cast<long long>(p->batch) * p->kv_heads;
+  const long long longest = (p->kv_len + kTileKeys - 1) / kTileKeys;
+  const long long tiles = lines * longest;
+  p->group_inv = 65536 / p->group + 1;
+  p->cluster_log2 = 0;
+  // Twice the CTAs while a warp has more than one tile and they fit in one wave:
+  // clusters of eight do not fill every GPC (16 of them took a second wave).
+  while (p->cluster_log2 < 3 && longest > kWarps << p->cluster_log2 &&
+         (lines << (p->cluster_log2 + 1)) * 8 <= sms * (p->cluster_log2 < 2 ? 7 : 6))
+    ++p->cluster_log2;
+  p->alone = lines <= sms &&
+             longest <= (kWarps * kAlone + (p->lens == nullptr ? tiles / sms : 0)) << p->cluster_log2;
+  if (p->alone) return static_cast<int>(lines << p->cluster_log2);
+  p->cluster_log2 = 0;
   return static_cast<int>(tiles < sms ? (tiles > 0 ? tiles : 1) : sms);
 }
 int kv8_rows_tile() { return kTileKeys; }

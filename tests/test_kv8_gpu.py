@@ -216,6 +216,29 @@ def test_attention_few_rows(ex, fmt, case):
     _assert_close(got, ref, bound)
 
 
+# How a line's keys are shared out follows from the number of lines and the longest one they may have.
+SHARES = [  # batch, q_len, heads, kv_heads, dim, capacity, lens, causal
+    (1, 1, 2, 1, 128, 1600, [1600], False),           # a cluster of CTAs to a line
+    (2, 3, 8, 4, 128, 1100, [1100, 37], True),
+    (4, 1, 8, 4, 64, 1000, [1000, 0, 33, 512], False),
+    (3, 2, 24, 8, 128, 700, [700, 31, 65], True),
+    (9, 1, 16, 8, 64, 500, [(61 * i) % 501 for i in range(9)], False),
+    (1, 1, 16, 1, 128, 12000, [11999], False),        # equal shares: one line over all CTAs
+    (2, 4, 8, 4, 64, 9000, [9000, 70], True),
+    (3, 1, 16, 8, 128, 8000, [8000, 1, 4001], False),
+    (2, 1, 16, 8, 128, 7000, [300, 0], False),        # lines that turn out short: a CTA to each
+    (3, 2, 12, 6, 128, 9000, [96, 700, 1], True),
+]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("case", SHARES, ids=[str(i) for i in range(len(SHARES))])
+def test_attention_few_rows_shares(ex, fmt, case):
+    batch, q_len, heads, kv_heads, dim, capacity, lens, causal = case
+    got, ref, bound = _attend(ex, fmt, batch, q_len, heads, kv_heads, dim, capacity, lens, causal)
+    _assert_close(got, ref, bound)
+
+
 MANY = [
     (1, 17, 1, 1, 128, 64, [40], False),
     (1, 128, 2, 1, 128, 128, [128], False),
@@ -285,7 +308,7 @@ def test_attention_nan_queries_stay_in_their_rows(ex, q_len):
     _assert_close(got, ref, bound)
 
 
-@pytest.mark.parametrize("q_len,kv_len", [(1, 4000), (6, 4000), (200, 1500)])
+@pytest.mark.parametrize("q_len,kv_len", [(1, 700), (1, 4000), (6, 4000), (1, 15000), (200, 1500)])
 def test_attention_is_repeatable_and_uses_its_stream(ex, q_len, kv_len):
     """The same bits on every call (split keys are joined in a fixed order), on another stream, into a strided output."""
     import torch
