@@ -403,9 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         // The tile is in registers: its stage takes the next load.
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && ua < u1) load(st);
+        if (u + kStages < u1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) load(st);
+        }
         if (++st == kStages) {
           st = 0;
           ph ^= 1u;
