@@ -192,9 +192,13 @@ struct Kv8AttnParams {
   unsigned int* count;  // arrivals per (sequence, kv head), zero between launches
   unsigned int* status;
   // Many rows (kv8_attn_plan): heads of a row line, row lines per sequence,
-  // pairs of query tiles per line, parts of the keys, work items.  `rows` is
-  // then the rows of a line.
-  int pack, pack_log2, lines, pairs, n_split, n_items;
+  // pairs of query tiles per line, pairs in all, key blocks of kv_len, CTAs.  Keys
+  // split over the CTAs: `parts` to a pair, or (parts 0) equal shares of `each`
+  // blocks, one more for the first `more` CTAs.
+  // `rows` is then the rows of a line.
+  int pack, pack_log2, lines, pairs, n_items, blocks, grid;
+  bool split;
+  int parts, each, more;
 };
 // Attention of up to 16 query rows over the cache (kv8_rows_sm100.cu); tk/tv are
 // ax_make_tmap_codes maps with boxes of kv8_rows_tile() rows.
@@ -209,7 +213,7 @@ cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const 
 bool kv8_attn_plan(Kv8AttnParams* p, int sms);  // false: too many items
 size_t kv8_attn_part_floats(const Kv8AttnParams& p);
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const CUtensorMap& to, const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream);
+                            const CUtensorMap& to, const Kv8AttnParams& p, int dev, cudaStream_t stream);
 
 // W8 (bits 8) / W4 (bits 4) codes + fp16 scale/zero per row and 64 columns ->
 // fp16 [rows][out_stride] (dequant_sm100.cu).

@@ -345,7 +345,7 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
     if (rc == ANIMAXS_OK)
       rc = ax_make_tmap_rows(ctx, &to, p.o, D, p.pack, p.q_len, p.lines, p.batch, p.o_tok, p.o_head, p.o_batch, 32);
     if (rc != ANIMAXS_OK) return rc;
-    e = ax::launch_kv8_attn(tq, tk, tv, to, p, ctx->num_sms, ctx->device, s);
+    e = ax::launch_kv8_attn(tq, tk, tv, to, p, ctx->device, s);
   }
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "attention launch");
   ctx->last_error.clear();

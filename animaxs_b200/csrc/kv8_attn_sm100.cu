@@ -171,11 +171,20 @@ struct alignas(16) Item {
 };
 static_assert(sizeof(Item) == 48, "items are read as three 16-byte words");
 
-__device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
+// Split keys, by parts: p.parts CTAs to each unit (pair of tiles).  By shares
+// (parts 0): the blocks of all units, p.blocks each as if none were shorter, in a
+// row; CTA c takes [share_begin(c), share_begin(c + 1)), which is less than a
+// unit and so touches at most two.
+__device__ __forceinline__ int share_begin(const Kv8AttnParams& p, int c) { return c * p.each + min(c, p.more); }
+__device__ __forceinline__ int share_owner(const Kv8AttnParams& p, int v) {
+  const int big = p.more * (p.each + 1);
+  return v < big ? v / (p.each + 1) : p.more + (v - big) / p.each;
+}
+
+// The part [lo, hi) of p.blocks of unit w; `part` is where its partial result goes.
+__device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w, int lo, int hi, int part) {
   Item it;
-  it.w = w;
-  const int s = w % p.n_split;
-  w /= p.n_split;
+  it.w = part;
   const int pair = p.causal ? p.pairs - 1 - w % p.pairs : w % p.pairs;  // the longest first
   w /= p.pairs;
   it.h = w % p.lines;
@@ -191,8 +200,10 @@ __device__ __forceinline__ Item kv8_item(const Kv8AttnParams& p, int w) {
   };
   const int a = blocks(it.q0), b = blocks(it.q0 + kTileM);
   const int n = max(a, b);
-  it.j0 = static_cast<int>(static_cast<long long>(n) * s / p.n_split);
-  const int j1 = static_cast<int>(static_cast<long long>(n) * (s + 1) / p.n_split);
+  // A shorter unit is cut in the same proportions.
+  const bool all = n == p.blocks || (lo == 0 && hi == p.blocks);
+  it.j0 = all ? lo : static_cast<int>(static_cast<long long>(n) * lo / p.blocks);
+  const int j1 = all ? min(hi, n) : static_cast<int>(static_cast<long long>(n) * hi / p.blocks);
   it.nA = max(min(a, j1) - it.j0, 0);
   it.nB = max(min(b, j1) - it.j0, 0);
   it.n = j1 - it.j0;
@@ -389,13 +400,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 14) {
       // --------------------------------------------------------- scheduler --
       if (lane == 0) {
-        uint32_t i = 0;
-        for (int w = w0;; w += wstep, ++i) {
-          const bool last = w >= p.n_items;
+        // Whole units round-robin, or a part of one, or a share's parts of one or two.
+        int v = 0, end = 0, w = w0;
+        if (p.split && p.parts > 0) {
+          w = w0 / p.parts;
+          const int k = w0 - w * p.parts;
+          v = w * p.blocks + p.blocks * k / p.parts;
+          end = w * p.blocks + p.blocks * (k + 1) / p.parts;
+        } else if (p.split) {
+          v = share_begin(p, w0);
+          end = share_begin(p, w0 + 1);
+          w = v / p.blocks;
+        }
+        for (uint32_t i = 0;; ++i) {
+          const bool last = p.split ? v >= end : w >= p.n_items;
           Item I;
-          if (!last)
-            I = kv8_item(p, w);
-          else
+          if (!last) {
+            const int lo = p.split ? v - w * p.blocks : 0, hi = p.split ? min(lo + end - v, p.blocks) : p.blocks;
+            I = kv8_item(p, w, lo, hi, 2 * w0 + static_cast<int>(i));
+            v += hi - lo;
+            w += p.split ? 1 : wstep;
+          } else
             I.q0 = I.h = I.b = I.kvh = I.len = I.j0 = I.nA = I.nB = I.n = 0, I.w = -1;
           const uint32_t e = i % kItems;
           if (!mbar_wait(BAR(kBarItemEmpty + e), ((i / kItems) & 1u) ^ 1u, abort_flag, p.status)) break;
@@ -600,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       gt += I.n;
       // A row without a visible key has m = -inf and l = 0; one with NaN scores has l = NaN.
       const bool none = nX == 0 || (m == -INFINITY && l == l);
-      if (p.n_split > 1) {
-        // [item][tile][HD / 4][128 rows] float4, then m and l of the rows.
+      if (p.split) {
+        // [part][tile][HD / 4][128 rows] float4, then m and l of the rows.
         float* part = p.part + (2LL * I.w + X) * (kTileM * (HD + 2));
         const bool live = row < p.rows;
         if (live) {
@@ -675,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #undef BAR
 }
 
-// Joins the n_split parts of every row in order: O = sum O'_s 2^(m_s - m) / sum l_s 2^(m_s - m).
+// Joins the parts of every row in order: O = sum O'_s 2^(m_s - m) / sum l_s 2^(m_s - m).
 // A thread takes 8 output values of a row; consecutive threads take consecutive rows.
 template <int HD>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
@@ -693,20 +718,42 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
   const int h = w / p.pairs % p.lines, b = w / p.pairs / p.lines;
   float m = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
-#pragma unroll 4
-  for (int s = 0; s < p.n_split; ++s) {
-    const float* part = p.part + (2LL * (static_cast<long long>(unit) * p.n_split + s) + X) * (kTileM * (HD + 2));
-    const float pm = __ldcg(part + kTileM * HD + t), pl = __ldcg(part + kTileM * HD + kTileM + t);
-    const float mn = fmaxf(m, pm);
-    const float fo = m == mn ? 1.f : ex2_approx(m - mn);
-    const float fn = pm == mn ? 1.f : ex2_approx(pm - mn);
-    m = mn;
-    l = l * fo + pl * fn;
-    if (pm == -INFINITY && pl == 0.f) continue;  // nothing stored (the first live part makes fo 0)
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8) * kTileM + t);
-    const float4 y = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8 + 1) * kTileM + t);
-    a = make_float4(a.x * fo + x.x * fn, a.y * fo + x.y * fn, a.z * fo + x.z * fn, a.w * fo + x.w * fn);
-    c = make_float4(c.x * fo + y.x * fn, c.y * fo + y.y * fn, c.z * fo + y.z * fn, c.w * fo + y.w * fn);
+  int first = unit * p.parts, n = p.parts;
+  bool second = false;  // of its CTA's parts, as a unit's first may be
+  if (n == 0) {
+    first = share_owner(p, unit * p.blocks);
+    n = share_owner(p, (unit + 1) * p.blocks - 1) - first + 1;
+    second = share_begin(p, first) < unit * p.blocks;
+  }
+  constexpr int kJoin = 4;
+  const float* part0 = p.part + (4LL * first + X) * (kTileM * (HD + 2));
+#pragma unroll 1
+  for (int s0 = 0; s0 < n; s0 += kJoin) {  // the loads of kJoin parts in flight
+    float pm[kJoin], pl[kJoin];
+    float4 x[kJoin], y[kJoin];
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const int s = s0 + i;
+      pm[i] = -INFINITY;
+      pl[i] = 0.f;
+      if (s >= n) continue;
+      const float* part = part0 + (4LL * s + (s == 0 && second ? 2 : 0)) * (kTileM * (HD + 2));
+      pm[i] = __ldcg(part + kTileM * HD + t);
+      pl[i] = __ldcg(part + kTileM * HD + kTileM + t);
+      x[i] = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8) * kTileM + t);
+      y[i] = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8 + 1) * kTileM + t);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      const float mn = fmaxf(m, pm[i]);
+      const float fo = m == mn ? 1.f : ex2_approx(m - mn);
+      const float fn = pm[i] == mn ? 1.f : ex2_approx(pm[i] - mn);
+      m = mn;
+      l = l * fo + pl[i] * fn;
+      if (pm[i] == -INFINITY && pl[i] == 0.f) continue;  // nothing stored (the first live part makes fo 0)
+      a = make_float4(a.x * fo + x[i].x * fn, a.y * fo + x[i].y * fn, a.z * fo + x[i].z * fn, a.w * fo + x[i].w * fn);
+      c = make_float4(c.x * fo + y[i].x * fn, c.y * fo + y[i].y * fn, c.z * fo + y[i].z * fn, c.w * fo + y[i].w * fn);
+    }
   }
   const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
   const int head = h * p.pack + row % p.pack;
@@ -728,17 +775,18 @@ cudaError_t launch_hd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
     configured.fetch_or(bit, std::memory_order_acq_rel);
   }
   cudaError_t e = launch_pdl(kernel, grid, kThreads, Smem<HD>::kBytes, stream, tq, tk, tv, to, p);
-  if (e == cudaSuccess && p.n_split > 1)
+  if (e == cudaSuccess && p.split)
     e = launch_pdl(kv8_join_kernel<HD>, p.batch * p.lines * p.pairs * 2 * (HD / 8), 128, 0, stream, p);
   return e;
 }
 
 }  // namespace
 
-// Fills in the rows, pairs and parts of a launch.  Parts: a pair of tiles over
-// all its keys is one item when the items fill the SMs; otherwise the keys are
-// cut into the number of parts for which the busiest SM has the least to do,
-// counting four key blocks' time for each item's start and end.
+// Fills in the rows, pairs and shares of a launch.  A pair of tiles over all its
+// keys is one item when the pairs fill the SMs; otherwise the keys are cut into
+// shares, whichever leaves the busiest SM the least to do: a whole number of
+// CTAs to each pair, or equal shares over all SMs.  Each item's start and end
+// counts as four key blocks' time.
 bool kv8_attn_plan(Kv8AttnParams* p, int sms) {
   p->pack = kTileM % p->group == 0 ? p->group : 1;
   p->pack_log2 = 0;
@@ -748,28 +796,35 @@ bool kv8_attn_plan(Kv8AttnParams* p, int sms) {
   p->pairs = (p->rows + 2 * kTileM - 1) / (2 * kTileM);
   const long long pairs = static_cast<long long>(p->batch) * p->lines * p->pairs;
   const long long blocks = (p->kv_len + kBlk - 1) / kBlk;
-  p->n_split = 1;
-  if (pairs < sms) {
-    long long best = 0;
-    for (int s = 1; s <= 32 && s <= blocks; ++s) {
-      const long long cost = (pairs * s + sms - 1) / sms * ((blocks + s - 1) / s + 4);
-      if (s == 1 || cost < best) {
-        best = cost;
-        p->n_split = s;
-      }
+  p->blocks = static_cast<int>(blocks);
+  long long ctas = 0;  // 0: not split
+  p->parts = 0;
+  if (pairs < sms && blocks * sms <= 0x7fffffffLL) {
+    long long best = blocks + 4;
+    for (long long n = 2; n <= blocks && pairs * n <= sms; ++n) {
+      const long long cost = (blocks + n - 1) / n + 4;
+      if (cost < best) best = cost, ctas = pairs * n, p->parts = static_cast<int>(n);
+    }
+    if (pairs * blocks >= sms && (pairs * blocks + sms - 1) / sms + 8 < best) {
+      ctas = sms;
+      p->parts = 0;
     }
   }
-  if (pairs * p->n_split > 0x7fffffffLL / (2 * 16)) return false;
-  p->n_items = static_cast<int>(pairs * p->n_split);
+  p->split = ctas != 0;
+  p->each = p->split ? static_cast<int>(pairs * blocks / ctas) : 0;
+  p->more = p->split ? static_cast<int>(pairs * blocks % ctas) : 0;
+  if (pairs > 0x7fffffffLL / (2 * 16)) return false;
+  p->n_items = static_cast<int>(pairs);
+  p->grid = static_cast<int>(p->split ? ctas : pairs < sms ? pairs : sms);
   return true;
 }
 size_t kv8_attn_part_floats(const Kv8AttnParams& p) {
-  return p.n_split > 1 ? 2 * static_cast<size_t>(p.n_items) * kTileM * (p.head_dim + 2) : 0;
+  return p.split ? 4 * static_cast<size_t>(p.grid) * kTileM * (p.head_dim + 2) : 0;
 }
 
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const CUtensorMap& to, const Kv8AttnParams& p, int sms, int dev, cudaStream_t stream) {
-  const int grid = p.n_items < sms ? p.n_items : sms;
+                            const CUtensorMap& to, const Kv8AttnParams& p, int dev, cudaStream_t stream) {
+  const int grid = p.grid;
   if (p.format == kKv8Int8)
     return p.head_dim == 128 ? launch_hd<kKv8Int8, 128>(tq, tk, tv, to, p, grid, dev, stream)
                              : launch_hd<kKv8Int8, 64>(tq, tk, tv, to, p, grid, dev, stream);
