@@ -249,6 +249,8 @@ MANY = [
     (1, 1024, 16, 16, 128, 512, [128], False),        # an image's queries on a padded context
     (1, 64, 16, 8, 128, 3000, [2999], True),          # a prompt chunk on a long cache
     (2, 40, 32, 2, 128, 1000, [1000, 321], True),     # a group of 16
+    (5, 300, 10, 10, 64, 2000, [2000, 0, 1999, 65, 700], True),   # equal shares of the keys over all SMs
+    (3, 290, 40, 20, 128, 1500, [1500, 1, 833], False),
 ]
 
 
