@@ -11,10 +11,10 @@
 // the group's heads (row = token * group + head), so that short chunks fill a
 // tile; otherwise every query head is on its own.
 //
-// A work item is a pair of query tiles (A, B) of one (sequence, head line) and,
-// when the pairs alone would leave SMs idle, one of n_split parts of their
-// keys; kv8_join_kernel then joins the parts in order.  Items are dealt
-// round-robin to one persistent CTA per SM.  Sixteen warps:
+// A work item is a pair of query tiles (A, B) of one (sequence, head line), dealt
+// round-robin to one persistent CTA per SM; where the pairs alone would leave
+// SMs idle, the keys are split over the CTAs (kv8_attn_plan) and kv8_join_kernel
+// joins the parts in order.  Sixteen warps:
 //   0-3, 4-7   softmax of tile A / B: thread t owns row t (= TMEM lane t)
 //   8-11       conversion of each K and V block
 //   12, 15     MMA issuers of tile A / B (12 owns TMEM); one warp for both spent
@@ -29,6 +29,18 @@
 // buffer of 128 keys each softmax waited 1200 of its 4300 cycles for
 // PV(j) and QK(j + 1).  O is rescaled only when a row's maximum grows by more
 // than 2^8.
+//
+// Measured (GPU time of a call in a graph): 4096 queries x 16 heads on up to 512
+// keys, batch 8 (int8) 103 us; 512 queries x 16 heads on 8704 keys, batch 2 (e4m3,
+// causal) 76 us = 930 TFLOP/s, 0.55 of the measured bf16 peak.  No unit is full:
+// tensor pipe 35 % of active cycles, exp2 32 %, ALU 33 %, shared memory 25 %, DRAM
+// 24 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  What
+// binds is the chain softmax -> P -> PV -> QK -> scores of each tile, about 1450
+// cycles a block with no work in it, of which two tiles in turn hide a part.
+// Slower, each measured: 128-key blocks (128 us for the first), a maximum taken a
+// block ahead (141), exponentials before the maximum is known (115), an epilogue
+// warpgroup of its own (111), e4m3 conversion on the ALU (95 against 83 then).
+//
 // Every wait is bounded; a timeout raises the CTA's abort flag and the status
 // bit, and the CTA drains and exits.
 #include <atomic>

@@ -4,6 +4,12 @@
 // Both are streams: 2 bytes in and 1 out per value (write), 1 in and 2 out
 // (read), so HBM bounds them when there is enough to move and the latency of
 // one dependent chain (positions -> rows -> maximum -> codes) when there is not.
+//
+// Measured (GPU time of a call in a graph, bytes moved over it; a copy reaches
+// 6.54 TB/s): write of 1 token x 8 heads x 8 sequences 2.35 us, of 8 x 512 tokens
+// x 16 heads 10.1 us = 4.97 TB/s, of 2 x up to 16385 tokens x 8 heads 20.2 us =
+// 5.95 TB/s; read of 32741 tokens x 8 heads 33.2 us = 6.07 TB/s.  The middle
+// sizes are a few waves of short CTAs, whose start and end are not hidden.
 #include "kernels.h"
 #include "kv8_common.cuh"
 #include "sm100_ptx.cuh"

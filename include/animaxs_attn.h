@@ -326,8 +326,10 @@ int animaxs_cross_kv_cache_reset(animaxs_cross_kv_cache* cache);
  *   k_scale, v_scale  fp32 [batch][kv_heads][ceil(capacity / 64)]
  * A value is code * scale of its head and 64-token block.  INT8 codes are
  * -127..127, E4M3 codes are 8-bit floats of magnitude <= 448.  The caller keeps
- * each sequence's length; what lies at or past it is never read, so neither
- * codes nor scales have to be initialised. */
+ * each sequence's length; what lies at or past it does not enter a result, so
+ * neither codes nor scales have to be initialised.  A length that counts
+ * positions not written yet (a padded batch of prompts, whose later keys a
+ * causal mask hides) needs finite values there, zeros for instance. */
 typedef enum animaxs_kv8_format { ANIMAXS_KV8_INT8 = 0, ANIMAXS_KV8_E4M3 = 1 } animaxs_kv8_format;
 
 #define ANIMAXS_KV8_BLOCK_TOKENS 64 /* tokens that share a scale */
