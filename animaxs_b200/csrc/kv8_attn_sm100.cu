@@ -34,9 +34,10 @@
 // keys, batch 8 (int8) 103 us; 512 queries x 16 heads on 8704 keys, batch 2 (e4m3,
 // causal) 76 us = 930 TFLOP/s, 0.55 of the measured bf16 peak.  No unit is full:
 // tensor pipe 35 % of active cycles, exp2 32 %, ALU 33 %, shared memory 25 %, DRAM
-// 24 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  What
-// binds is the chain softmax -> P -> PV -> QK -> scores of each tile, about 1450
-// cycles a block with no work in it, of which two tiles in turn hide a part.
+// 24 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  Of 2060
+// cycles a block (clocks in the kernel) a softmax warp works 1840 (maximum 430,
+// exponentials and P 1130: two tiles share the exp2 unit, 1024), an MMA warp 1425
+// (QK at N = 64 reads 6 KB of shared memory per 32 cycles of MMA).
 // Slower, each measured: 128-key blocks (128 us for the first), a maximum taken a
 // block ahead (141), exponentials before the maximum is known (115), an epilogue
 // warpgroup of its own (111), e4m3 conversion on the ALU (95 against 83 then).
