@@ -185,7 +185,9 @@ class QuantizedKVCache:
         import torch
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)  # 1 us less than new_empty
-        key = ("a", q.shape, q.stride(), out.shape, out.stride(), kv_len, causal, scale, qk_norm, eps)
+            key = ("a", q.shape, q.stride(), kv_len, causal, scale, qk_norm, eps)
+        else:
+            key = ("o", q.shape, q.stride(), kv_len, causal, scale, qk_norm, eps, out.shape, out.stride())
         d = self._descs.get(key)
         if d is None:
             self._view(q, None, q.shape[2] if q.dim() == 4 else 0, "q")
