@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float nk = 0.f, nv = 0.f;  // thread 0: scales of the next K block
     auto scales = [&](const Item& I, int j) {
       const long long at = (static_cast<long long>(I.b) * p.kv_heads + I.kvh) * p.n_blocks + I.j0 + j;
-      nk = __ldg(p.k_scale + at);
-      nv = __ldg(p.v_scale + at);
+      nk = p.k_scale[at];
+      nv = p.v_scale[at];
     };
     while (true) {
       const Item I = next_item(false, ok);
@@ -751,10 +751,10 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8AttnParams p) {
       pl[i] = 0.f;
       if (s >= n) continue;
       const float* part = part0 + (4LL * s + (s == 0 && second ? 2 : 0)) * (kTileM * (HD + 2));
-      pm[i] = __ldcg(part + kTileM * HD + t);
-      pl[i] = __ldcg(part + kTileM * HD + kTileM + t);
-      x[i] = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8) * kTileM + t);
-      y[i] = __ldcg(reinterpret_cast<const float4*>(part) + (2 * d8 + 1) * kTileM + t);
+      pm[i] = part[kTileM * HD + t];
+      pl[i] = part[kTileM * HD + kTileM + t];
+      x[i] = reinterpret_cast<const float4*>(part)[(2 * d8) * kTileM + t];
+      y[i] = reinterpret_cast<const float4*>(part)[(2 * d8 + 1) * kTileM + t];
     }
 #pragma unroll
     for (int i = 0; i < kJoin; ++i) {

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = row0 + i * kRowsPerPass;
-    if (r >= lo && r < hi) x[i] = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+    if (r >= lo && r < hi) x[i] = *reinterpret_cast<const uint4*>(src + r * p.tok[kv]);
   }
   // Largest magnitude; NaN and infinity show in it and send the thread to the
   // slower form (most of the kernel's instructions are per value, and it is
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
     for (int i = 0; i < kPasses; ++i) {
       const int r = row0 + i * kRowsPerPass;
       if (r >= lo && r < hi) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+        const uint4 v = *reinterpret_cast<const uint4*>(src + r * p.tok[kv]);
         mx = __hmax2(mx, __hmax2(__hmax2(finite_abs(v.x), finite_abs(v.y)), __hmax2(finite_abs(v.z), finite_abs(v.w))));
       }
     }
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
     for (int i = 0; i < kPasses; ++i) {
       const int r = row0 + i * kRowsPerPass;
       if (r >= lo && r < hi) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + r * p.tok[kv]));
+        const uint4 v = *reinterpret_cast<const uint4*>(src + r * p.tok[kv]);
         uint2 c = make_uint2(0u, 0u);
         if (inv > 0.f) c = make_uint2(quantise4<FMT, false>(v.x, v.y, inv), quantise4<FMT, false>(v.z, v.w, inv));
         *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * HD) = c;
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadPar
     c[i] = make_uint2(0u, 0u);
     s[i] = 0.f;
     if (t < p.tokens && pos < len) {
-      c[i] = __ldg(reinterpret_cast<const uint2*>(codes + static_cast<long long>(pos) * HD));
-      s[i] = __ldg(scale + pos / kKv8Block);
+      c[i] = *reinterpret_cast<const uint2*>(codes + static_cast<long long>(pos) * HD);
+      s[i] = scale[pos / kKv8Block];
     }
   }
 #pragma unroll

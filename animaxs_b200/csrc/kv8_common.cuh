@@ -71,7 +71,10 @@ __device__ __forceinline__ uint32_t kv8_pack4(float a, float b, float c, float d
 // Programmatic dependent launch: the kernels of the cache follow one another
 // (a step writes, then attends), so each may be set up while the one before it
 // ends.  pdl_wait() returns when that one has completed and its writes are
-// visible; nothing of global memory is touched before it.
+// visible; nothing of global memory is touched before it.  What a predecessor may
+// have written (lengths, scales, codes, q, k, v, partial results) is read by
+// ordinary loads: the non-coherent ones (__ldg) are for data that nobody writes
+// while the kernel is resident, and may be moved across the wait.
 __device__ __forceinline__ void pdl_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -103,7 +106,7 @@ cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned thread
 
 // A sequence's length, within [0, kv_len].
 __device__ __forceinline__ int kv8_len(const int* lens, int kv_valid, int kv_len, int b) {
-  const int n = lens != nullptr ? __ldg(lens + b) : kv_valid;
+  const int n = lens != nullptr ? lens[b] : kv_valid;
   return min(max(n, 0), kv_len);
 }
 

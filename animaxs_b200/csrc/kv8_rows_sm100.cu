@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto scales = [&](const Place& s, float& k, float& v) {
       const long long idx =
           (static_cast<long long>(s.b) * p.kv_heads + s.h) * p.n_blocks + s.tile / (kKv8Block / kTileKeys);
-      k = __ldg(p.k_scale + idx);
-      v = __ldg(p.v_scale + idx);
+      k = p.k_scale[idx];
+      v = p.v_scale[idx];
     };
     Place nx = at;  // the next tile's place, whose scales are loaded ahead
     float sk_next, sv_next;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                             c * (HD / 4));
 #pragma unroll
           for (int k = 0; k < HD / 32; ++k) {
-            const uint4 v = __ldg(src + k);
+            const uint4 v = src[k];
             qf[nt][2 * k][0] = v.x;
             qf[nt][2 * k][1] = v.y;
             qf[nt][2 * k + 1][0] = v.z;
