@@ -27,10 +27,11 @@ struct animaxs_attn_ctx {
   size_t scratch_bytes = 0;
   void* staging = nullptr;        // head-sharded path: per-rank slice + gather buffer
   size_t staging_bytes = 0;
-  float* kv8_part = nullptr;           // partial results of split 8-bit-cache attention
-  size_t kv8_part_bytes = 0;
-  unsigned int* kv8_count = nullptr;   // arrivals per split item, zero between calls
-  size_t kv8_count_n = 0;
+  // Workspaces of split 8-bit-cache attention, each made at its first use as large
+  // as any call on this device needs and never moved: captured graphs point at them.
+  float* kv8_rows_part = nullptr;      // few rows: partial results
+  unsigned int* kv8_count = nullptr;   // few rows: arrivals [num_sms], zero between calls
+  float* kv8_tile_part = nullptr;      // many rows: partial results
   unsigned int* d_status = nullptr;  // device status word written by kernels
   int64_t query_tiles = 0;
   bool timing = false;                        // bracket each attention kernel with events

@@ -107,8 +107,9 @@ extern "C" int animaxs_attn_destroy(animaxs_attn_ctx* ctx) {
   cudaDeviceSynchronize();
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->staging) cudaFree(ctx->staging);
-  if (ctx->kv8_part) cudaFree(ctx->kv8_part);
+  if (ctx->kv8_rows_part) cudaFree(ctx->kv8_rows_part);
   if (ctx->kv8_count) cudaFree(ctx->kv8_count);
+  if (ctx->kv8_tile_part) cudaFree(ctx->kv8_tile_part);
   if (ctx->d_status) cudaFree(ctx->d_status);
   for (cudaEvent_t e : ctx->events) cudaEventDestroy(e);
   cudaSetDevice(prev);
@@ -550,7 +551,7 @@ extern "C" int animaxs_attn_synchronize(animaxs_attn_ctx* ctx, void* stream) {
   if (e == cudaSuccess && status != 0) e = cudaMemset(ctx->d_status, 0, sizeof(status));
   // A kernel that gave up may have left arrivals of a split item uncounted.
   if (e == cudaSuccess && status != 0 && ctx->kv8_count != nullptr)
-    e = cudaMemset(ctx->kv8_count, 0, ctx->kv8_count_n * sizeof(unsigned int));
+    e = cudaMemset(ctx->kv8_count, 0, ctx->num_sms * sizeof(unsigned int));
   cudaSetDevice(prev);
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "synchronize");
   if (status & ax::kStatusTimeoutBit)

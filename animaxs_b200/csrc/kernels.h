@@ -189,7 +189,7 @@ struct Kv8AttnParams {
   bool alone;
   int cluster_log2, group_inv;
   float* part;          // workspace: partial results (kv8_rows_part_floats, kv8_attn_part_floats)
-  unsigned int* count;  // arrivals per (sequence, kv head), zero between launches
+  unsigned int* count;  // arrivals at a line that crosses CTAs, by the CTA it starts in; zero between launches
   unsigned int* status;
   // Many rows (kv8_attn_plan): heads of a row line, row lines per sequence,
   // pairs of query tiles per line, pairs in all, key blocks of kv_len, CTAs.  Keys
@@ -211,7 +211,7 @@ cudaError_t launch_kv8_rows(const CUtensorMap& tk, const CUtensorMap& tv, const 
 // Attention over the cache in pairs of 128-row query tiles (kv8_attn_sm100.cu);
 // tk/tv have 64-row boxes, tq and to are ax_make_tmap_rows maps of 128 and 32 rows.
 bool kv8_attn_plan(Kv8AttnParams* p, int sms);  // false: too many items
-size_t kv8_attn_part_floats(const Kv8AttnParams& p);
+size_t kv8_attn_part_floats(int head_dim, int grid);
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                             const CUtensorMap& to, const Kv8AttnParams& p, int dev, cudaStream_t stream);
 

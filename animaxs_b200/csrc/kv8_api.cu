@@ -118,32 +118,34 @@ int check_attn(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c, const animaxs_
   return ANIMAXS_OK;
 }
 
-// Workspace of split attention: `floats` of partial results and `counts`
-// arrival words, which stay zero between calls.
-int ensure_split(animaxs_attn_ctx* ctx, size_t floats, size_t counts) {
-  if (floats * sizeof(float) > ctx->kv8_part_bytes || counts > ctx->kv8_count_n) {
-    // The previous buffers may still be in use by queued work on another stream.
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess && floats * sizeof(float) > ctx->kv8_part_bytes) {
-      cudaFree(ctx->kv8_part);
-      ctx->kv8_part = nullptr;
-      ctx->kv8_part_bytes = 0;
-      e = cudaMalloc(&ctx->kv8_part, floats * sizeof(float));
-      if (e == cudaSuccess) ctx->kv8_part_bytes = floats * sizeof(float);
-    }
-    if (e == cudaSuccess && counts > ctx->kv8_count_n) {
-      cudaFree(ctx->kv8_count);
-      ctx->kv8_count = nullptr;
-      ctx->kv8_count_n = 0;
-      const size_t n = counts < 16384 ? 16384 : counts;
-      e = cudaMalloc(&ctx->kv8_count, n * sizeof(unsigned int));
-      if (e == cudaSuccess) e = cudaMemset(ctx->kv8_count, 0, n * sizeof(unsigned int));
-      if (e == cudaSuccess) e = cudaDeviceSynchronize();  // before work on a non-blocking stream counts
-      if (e == cudaSuccess) ctx->kv8_count_n = n;
-    }
-    if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "8-bit K/V cache attention workspace");
+// Workspaces of split attention.  Launches have one CTA per SM at most, which
+// bounds both: 2.5 MB for few rows, 39 MB for many.
+int ensure_rows_workspace(animaxs_attn_ctx* ctx) {
+  if (ctx->kv8_count != nullptr) return ANIMAXS_OK;
+  const size_t counts = ctx->num_sms * sizeof(unsigned int);
+  unsigned int* count = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (ctx->kv8_rows_part == nullptr) {
+    e = cudaMalloc(&ctx->kv8_rows_part, ax::kv8_rows_part_floats(128, ctx->num_sms) * sizeof(float));
+    if (e != cudaSuccess) ctx->kv8_rows_part = nullptr;
   }
+  if (e == cudaSuccess) e = cudaMalloc(&count, counts);
+  if (e == cudaSuccess) e = cudaMemset(count, 0, counts);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();  // before work on a non-blocking stream counts
+  if (e != cudaSuccess) {
+    if (count != nullptr) cudaFree(count);
+    return ax_cuda_fail(ctx, e, "8-bit K/V cache attention workspace");
+  }
+  ctx->kv8_count = count;
   return ANIMAXS_OK;
+}
+int ensure_tile_workspace(animaxs_attn_ctx* ctx) {
+  if (ctx->kv8_tile_part != nullptr) return ANIMAXS_OK;
+  const cudaError_t e =
+      cudaMalloc(&ctx->kv8_tile_part, ax::kv8_attn_part_floats(128, ctx->num_sms) * sizeof(float));
+  if (e == cudaSuccess) return ANIMAXS_OK;
+  ctx->kv8_tile_part = nullptr;
+  return ax_cuda_fail(ctx, e, "8-bit K/V cache attention workspace");
 }
 
 }  // namespace
@@ -332,17 +334,17 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   cudaError_t e;
   if (few) {
     const int grid = ax::kv8_rows_plan(&p, ctx->num_sms);
-    rc = ensure_split(ctx, ax::kv8_rows_part_floats(d->head_dim, grid), static_cast<size_t>(heads));
+    rc = ensure_rows_workspace(ctx);
     if (rc != ANIMAXS_OK) return rc;
-    p.part = ctx->kv8_part;
+    p.part = ctx->kv8_rows_part;
     p.count = ctx->kv8_count;
     e = ax::launch_kv8_rows(tk, tv, p, grid, ctx->device, s);
   } else {
     if (!ax::kv8_attn_plan(&p, ctx->num_sms))
       return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "attention byte size overflow");
-    rc = ensure_split(ctx, ax::kv8_attn_part_floats(p), 0);
+    if (p.split) rc = ensure_tile_workspace(ctx);
     if (rc != ANIMAXS_OK) return rc;
-    p.part = ctx->kv8_part;
+    p.part = ctx->kv8_tile_part;
     rc = ax_make_tmap_rows(ctx, &tq, p.q, D, p.pack, p.q_len, p.lines, p.batch, p.q_tok, p.q_head, p.q_batch,
                            ax::kTileM);
     if (rc == ANIMAXS_OK)

@@ -831,8 +831,8 @@ bool kv8_attn_plan(Kv8AttnParams* p, int sms) {
   p->grid = static_cast<int>(p->split ? ctas : pairs < sms ? pairs : sms);
   return true;
 }
-size_t kv8_attn_part_floats(const Kv8AttnParams& p) {
-  return p.split ? 4 * static_cast<size_t>(p.grid) * kTileM * (p.head_dim + 2) : 0;
+size_t kv8_attn_part_floats(int head_dim, int grid) {
+  return 4 * static_cast<size_t>(grid) * kTileM * (head_dim + 2);
 }
 
 cudaError_t launch_kv8_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,

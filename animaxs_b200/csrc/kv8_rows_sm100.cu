@@ -729,8 +729,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int parts = 0;  // of the line, if this CTA has to join them
     if (ends[threadIdx.x] >= 0) {
       const SlotInfo at = info[ends[threadIdx.x]];
-      const int n = owner(at.line + at.tiles - 1) - owner(at.line) + 1;
-      unsigned* count = p.count + static_cast<long long>(at.b) * p.kv_heads + at.h;
+      // Of the lines that start in a CTA only its last one can go on behind it.
+      const int first = owner(at.line);
+      const int n = owner(at.line + at.tiles - 1) - first + 1;
+      unsigned* count = p.count + first;
       unsigned was;
       asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(was) : "l"(count) : "memory");
       if (static_cast<int>(was) == n - 1) {
