@@ -20,13 +20,19 @@ struct AxRange {
   AxRange& operator=(const AxRange&) = delete;
 };
 
+// A device buffer of the context that grows on demand (ax_grow_buffer).
+struct AxBuffer {
+  void* ptr = nullptr;
+  size_t bytes = 0;
+  bool captured = false;  // a call in stream capture used it: a graph may hold its address
+};
+
 struct animaxs_attn_ctx {
   int device = 0;
   int num_sms = 0;
-  void* scratch = nullptr;        // normalised q/k copies (grown on demand)
-  size_t scratch_bytes = 0;
-  void* staging = nullptr;        // head-sharded path: per-rank slice + gather buffer
-  size_t staging_bytes = 0;
+  AxBuffer scratch;               // normalised q/k copies, decoded weights, re-laid RoPE tables
+  AxBuffer staging;               // head-sharded path: per-rank slice + gather buffer
+  std::vector<void*> retired;     // outgrown buffers that captured graphs may point at
   // Workspaces of split 8-bit-cache attention, each made at its first use as large
   // as any call on this device needs and never moved: captured graphs point at them.
   float* kv8_rows_part = nullptr;      // few rows: partial results
@@ -51,7 +57,10 @@ struct AxOutView {
 
 int ax_set_error(animaxs_attn_ctx* ctx, int code, const char* fmt, ...);
 int ax_cuda_fail(animaxs_attn_ctx* ctx, cudaError_t e, const char* what);
-int ax_ensure_scratch(animaxs_attn_ctx* ctx, size_t bytes);  // context scratch of at least `bytes`
+// At least `bytes` in `buffer` for a call on `stream`; an outgrown buffer that a graph may
+// hold lives until the context is destroyed.
+int ax_grow_buffer(animaxs_attn_ctx* ctx, AxBuffer* buffer, size_t bytes, cudaStream_t stream, const char* what);
+int ax_ensure_scratch(animaxs_attn_ctx* ctx, size_t bytes, cudaStream_t stream);
 int ax_validate(animaxs_attn_ctx* ctx, const animaxs_attn_desc* d, const void* q, const void* k,
                 const void* v, const void* o);
 int ax_make_tmap(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,

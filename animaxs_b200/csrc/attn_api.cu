@@ -47,25 +47,37 @@ int ax_cuda_fail(animaxs_attn_ctx* ctx, cudaError_t e, const char* what) {
   return ax_set_error(ctx, ANIMAXS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-int ax_ensure_scratch(animaxs_attn_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return ANIMAXS_OK;
-  if (ctx->scratch != nullptr) {
-    // The previous buffer may still be read by queued work on another stream.
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "scratch resize sync");
-    cudaFree(ctx->scratch);
-    ctx->scratch = nullptr;
-    ctx->scratch_bytes = 0;
+int ax_grow_buffer(animaxs_attn_ctx* ctx, AxBuffer* buffer, size_t bytes, cudaStream_t stream, const char* what) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(stream, &capture);
+  if (e != cudaSuccess) return ax_cuda_fail(ctx, e, what);
+  const bool capturing = capture != cudaStreamCaptureStatusNone;
+  if (bytes > buffer->bytes) {
+    if (buffer->ptr != nullptr && (buffer->captured || capturing)) {
+      ctx->retired.push_back(buffer->ptr);
+    } else if (buffer->ptr != nullptr) {
+      // The previous buffer may still be read by queued work on another stream.
+      e = cudaDeviceSynchronize();
+      if (e != cudaSuccess) return ax_cuda_fail(ctx, e, what);
+      cudaFree(buffer->ptr);
+    }
+    *buffer = AxBuffer{};
+    void* grown = nullptr;
+    e = cudaMalloc(&grown, bytes);
+    if (e != cudaSuccess) return ax_cuda_fail(ctx, e, what);
+    buffer->ptr = grown;
+    buffer->bytes = bytes;
   }
-  size_t grow = bytes + bytes / 8;
-  grow = (grow + 4095) & ~static_cast<size_t>(4095);
-  cudaError_t e = cudaMalloc(&ctx->scratch, grow);
-  if (e != cudaSuccess) {
-    ctx->scratch = nullptr;
-    return ax_cuda_fail(ctx, e, "scratch allocation");
-  }
-  ctx->scratch_bytes = grow;
+  buffer->captured |= capturing;
   return ANIMAXS_OK;
+}
+
+int ax_ensure_scratch(animaxs_attn_ctx* ctx, size_t bytes, cudaStream_t stream) {
+  if (bytes > ctx->scratch.bytes) {
+    bytes += bytes / 8;
+    bytes = (bytes + 4095) & ~static_cast<size_t>(4095);
+  }
+  return ax_grow_buffer(ctx, &ctx->scratch, bytes, stream, "scratch allocation");
 }
 
 extern "C" int animaxs_attn_abi_version(void) { return ANIMAXS_ATTN_ABI_VERSION; }
@@ -105,8 +117,9 @@ extern "C" int animaxs_attn_destroy(animaxs_attn_ctx* ctx) {
   cudaGetDevice(&prev);
   cudaSetDevice(ctx->device);
   cudaDeviceSynchronize();
-  if (ctx->scratch) cudaFree(ctx->scratch);
-  if (ctx->staging) cudaFree(ctx->staging);
+  if (ctx->scratch.ptr) cudaFree(ctx->scratch.ptr);
+  if (ctx->staging.ptr) cudaFree(ctx->staging.ptr);
+  for (void* p : ctx->retired) cudaFree(p);
   if (ctx->kv8_rows_part) cudaFree(ctx->kv8_rows_part);
   if (ctx->kv8_count) cudaFree(ctx->kv8_count);
   if (ctx->kv8_tile_part) cudaFree(ctx->kv8_tile_part);
@@ -394,10 +407,10 @@ int ax_forward_range(animaxs_attn_ctx* ctx, const animaxs_attn_desc* d, const vo
     // Layout as animaxs_attn_scratch_bytes counts it: q's copy, then k's at
     // the next 256-byte boundary (each only when the prologue writes it).
     const int64_t k_off = ((norm_q ? q_bytes : 0) + 255) & ~static_cast<int64_t>(255);
-    int rc = ax_ensure_scratch(ctx, static_cast<size_t>(k_off + (norm_k ? k_bytes : 0)));
+    int rc = ax_ensure_scratch(ctx, static_cast<size_t>(k_off + (norm_k ? k_bytes : 0)), stream);
     if (rc != ANIMAXS_OK) return rc;
-    __half* qn = static_cast<__half*>(ctx->scratch);
-    __half* kn = reinterpret_cast<__half*>(static_cast<char*>(ctx->scratch) + k_off);
+    __half* qn = static_cast<__half*>(ctx->scratch.ptr);
+    __half* kn = reinterpret_cast<__half*>(static_cast<char*>(ctx->scratch.ptr) + k_off);
     NormParams np{};
     np.head_dim = static_cast<int>(d->head_dim);
     np.eps = d->eps > 0.f ? d->eps : 1e-6f;

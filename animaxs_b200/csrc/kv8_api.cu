@@ -292,7 +292,7 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   p.rows = p.group * p.q_len;
   if (d->qk_norm == ANIMAXS_QK_RMS) {
     // q normalised into context scratch, by the kernel that normalises for animaxs_attn_forward.
-    rc = ax_ensure_scratch(ctx, static_cast<size_t>(d->batch) * d->q_len * d->heads * D * 2);
+    rc = ax_ensure_scratch(ctx, static_cast<size_t>(d->batch) * d->q_len * d->heads * D * 2, s);
     if (rc != ANIMAXS_OK) return rc;
     ax::NormParams np{};
     np.head_dim = d->head_dim;
@@ -301,7 +301,7 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
     np.status = ctx->d_status;
     ax::NormJob& j = np.job[0];
     j.in = p.q;
-    j.out = static_cast<__half*>(ctx->scratch);
+    j.out = static_cast<__half*>(ctx->scratch.ptr);
     j.in_tok = p.q_tok;
     j.in_head = p.q_head;
     j.in_batch = p.q_batch;

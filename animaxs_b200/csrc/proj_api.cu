@@ -192,7 +192,7 @@ extern "C" int animaxs_proj_forward(animaxs_attn_ctx* ctx, const animaxs_proj_de
   const size_t rope_bytes = rope ? (static_cast<size_t>(d->tokens) * 64 * 8 + 255) / 256 * 256 : 0;
   const size_t wdec_bytes = quant ? static_cast<size_t>(d->n) * d->k * 2 : 0;
   if (rope || quant) {
-    rc = ax_ensure_scratch(ctx, rope_bytes + wdec_bytes);
+    rc = ax_ensure_scratch(ctx, rope_bytes + wdec_bytes, static_cast<cudaStream_t>(stream));
     if (rc != ANIMAXS_OK) return rc;
   }
   const void* wmat = w;
@@ -200,7 +200,7 @@ extern "C" int animaxs_proj_forward(animaxs_attn_ctx* ctx, const animaxs_proj_de
   if (quant) {
     // Decode the W8/W4 weight into fp16 (ordered before the GEMM on the same
     // stream), as the reference's dequantize-then-GEMM path.
-    void* wdec = static_cast<char*>(ctx->scratch) + rope_bytes;
+    void* wdec = static_cast<char*>(ctx->scratch.ptr) + rope_bytes;
     cudaError_t e = ax::launch_dequant(d->w_storage == ANIMAXS_WEIGHT_W4 ? 4 : 8, w, d->w_scale, d->w_zero, wdec,
                                        d->n, d->k, d->w_packed_stride, d->k, ctx->num_sms,
                                        static_cast<cudaStream_t>(stream));
@@ -232,9 +232,9 @@ extern "C" int animaxs_proj_forward(animaxs_attn_ctx* ctx, const animaxs_proj_de
   if (rope) {
     // The epilogue reads the table pair-major: re-lay the `tokens` rows it uses
     // out into context scratch (ordered before the GEMM on the same stream).
-    cudaError_t e = ax::launch_rope_pairs(d->rope_table, ctx->scratch, d->tokens, static_cast<cudaStream_t>(stream));
+    cudaError_t e = ax::launch_rope_pairs(d->rope_table, ctx->scratch.ptr, d->tokens, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "rope table re-layout");
-    p.rope = static_cast<const float*>(ctx->scratch);
+    p.rope = static_cast<const float*>(ctx->scratch.ptr);
   }
   p.eps = d->eps > 0.f ? d->eps : 1e-6f;
   p.gate = d->gate;

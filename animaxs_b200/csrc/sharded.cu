@@ -205,22 +205,13 @@ extern "C" int animaxs_attn_forward_head_sharded(animaxs_attn_ctx* ctx, animaxs_
     view = AxOutView{o, d->o_tok_stride, d->o_head_stride, d->o_batch_stride, 0};
   } else {
     const size_t need = slice * world * sizeof(__half);
-    if (need > ctx->staging_bytes) {
-      int prev = 0;
-      cudaGetDevice(&prev);
-      cudaSetDevice(ctx->device);
-      if (ctx->staging) {
-        cudaDeviceSynchronize();
-        cudaFree(ctx->staging);
-        ctx->staging = nullptr;
-        ctx->staging_bytes = 0;
-      }
-      cudaError_t e = cudaMalloc(&ctx->staging, need);
-      cudaSetDevice(prev);
-      if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "staging allocation");
-      ctx->staging_bytes = need;
-    }
-    gather = static_cast<__half*>(ctx->staging);
+    int prev = 0;
+    cudaGetDevice(&prev);
+    cudaSetDevice(ctx->device);
+    rc = ax_grow_buffer(ctx, &ctx->staging, need, stream, "staging allocation");
+    cudaSetDevice(prev);
+    if (rc != ANIMAXS_OK) return rc;
+    gather = static_cast<__half*>(ctx->staging.ptr);
     view = AxOutView{gather + rank * slice, hr * D, D, static_cast<int64_t>(d->q_len) * hr * D, h0};
   }
   rc = ax_forward_range(ctx, d, q, k, v, o, h0, hr, &view, stream);

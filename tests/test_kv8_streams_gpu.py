@@ -124,3 +124,46 @@ def test_launches_of_different_shares_alternate(ex):
         for o, w in zip(outs, want):
             differ += (o.view(torch.int16) != w.view(torch.int16)).any()
     assert int(differ) == 0
+
+
+def test_a_graph_outlives_larger_scratch(ex):
+    """The context's scratch (normalised q, decoded weights) of a captured call, outgrown twice before the replay."""
+    import torch
+    cache = _filled(ex, 1, 1, 700, 8, 128)
+    q, w = _draw(2, 1, 40, 8, 128), _draw(3, 128)
+    out = torch.zeros_like(q)
+    graph = _capture(lambda: cache.attention(q, out, qk_norm="rms", q_norm_weight=w))
+    graph.replay()
+    first = out.clone()
+    plain = _draw(4, 1, 300, 16, 128)
+    self_out = torch.zeros_like(plain)
+    self_graph = _capture(lambda: ex.attention(plain, plain, plain, self_out, qk_norm="rms"))  # a larger scratch
+    self_graph.replay()
+    self_first = self_out.clone()
+    big = _draw(5, 1, 3000, 8, 128)
+    want = cache.attention(big, qk_norm="rms", q_norm_weight=w)                               # larger again
+    taken = [torch.full((1 << 20,), 7.0, dtype=torch.float16, device="cuda") for _ in range(8)]
+    for _ in range(3):
+        out.zero_()
+        self_out.zero_()
+        graph.replay()
+        self_graph.replay()
+        assert torch.equal(out, first) and torch.equal(self_out, self_first)
+        assert torch.equal(cache.attention(big, qk_norm="rms", q_norm_weight=w), want)
+    assert all((t == 7).all() for t in taken)
+
+
+def test_scratch_that_no_graph_holds_is_given_back(ex):
+    """Eager calls of growing size keep one scratch buffer, not all of them: six sizes up to 96 MB, in 200 MB."""
+    import torch
+    torch.cuda.synchronize()
+    qs = [torch.zeros((1, 4096 * n, 16, 128), dtype=torch.float16, device="cuda") for n in (1, 2, 3, 4, 5, 6)]
+    k = torch.zeros((1, 64, 16, 128), dtype=torch.float16, device="cuda")
+    out = torch.empty_like(qs[-1])
+    ex.attention(qs[0], k, k, out[:, :4096], qk_norm="rms", qk_norm_targets="q")
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for n, q in enumerate(qs, 1):
+        ex.attention(q, k, k, out[:, :4096 * n], qk_norm="rms", qk_norm_targets="q")
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] < 200 << 20
