@@ -558,13 +558,19 @@ extern "C" int animaxs_attn_synchronize(animaxs_attn_ctx* ctx, void* stream) {
   int prev = 0;
   cudaGetDevice(&prev);
   cudaSetDevice(ctx->device);
-  cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+  // All on the caller's stream: the legacy stream is not ordered with non-blocking
+  // ones, so that a reset there could land in the middle of the next call.
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
   unsigned int status = 0;
-  if (e == cudaSuccess) e = cudaMemcpy(&status, ctx->d_status, sizeof(status), cudaMemcpyDeviceToHost);
-  if (e == cudaSuccess && status != 0) e = cudaMemset(ctx->d_status, 0, sizeof(status));
-  // A kernel that gave up may have left arrivals of a split item uncounted.
-  if (e == cudaSuccess && status != 0 && ctx->kv8_count != nullptr)
-    e = cudaMemset(ctx->kv8_count, 0, ctx->num_sms * sizeof(unsigned int));
+  cudaError_t e = cudaMemcpyAsync(&status, ctx->d_status, sizeof(status), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && status != 0) {
+    e = cudaMemsetAsync(ctx->d_status, 0, sizeof(status), s);
+    // A kernel that gave up may have left arrivals of a split item uncounted.
+    if (e == cudaSuccess && ctx->kv8_count != nullptr)
+      e = cudaMemsetAsync(ctx->kv8_count, 0, ctx->num_sms * sizeof(unsigned int), s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
   cudaSetDevice(prev);
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "synchronize");
   if (status & ax::kStatusTimeoutBit)

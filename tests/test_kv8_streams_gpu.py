@@ -167,3 +167,35 @@ def test_scratch_that_no_graph_holds_is_given_back(ex):
         ex.attention(q, k, k, out[:, :4096 * n], qk_norm="rms", qk_norm_targets="q")
     torch.cuda.synchronize()
     assert free - torch.cuda.mem_get_info()[0] < 200 << 20
+
+
+def test_a_timeout_is_cleared_on_the_callers_stream(ex):
+    """A wait that runs out (1 ms, on a phase that nothing completes) on a non-blocking stream while the legacy stream
+    is busy: it is reported and cleared without waiting for the other stream, and the split attention that follows
+    at once has the right bits."""
+    import torch
+
+    from animaxs_b200 import AttentionTimeoutError
+    step, out = _decoding_step(ex)
+    step()
+    want = out.clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert ex._lib.animaxs_attn_selftest_wait_timeout(ex.handle, 1_000_000, side.cuda_stream) == 0
+    with pytest.raises(AttentionTimeoutError):             # a kernel's first launch loads it, which waits for the device
+        ex.synchronize(side)
+    torch.cuda._sleep(1_000_000_000)                       # about half a second on the legacy stream
+    busy = torch.cuda.Event()
+    busy.record()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            assert ex._lib.animaxs_attn_selftest_wait_timeout(ex.handle, 1_000_000, side.cuda_stream) == 0
+            with pytest.raises(AttentionTimeoutError):
+                ex.synchronize(side)
+            for _ in range(20):
+                step()
+            ex.synchronize(side)                           # the status is clear again
+            waited = busy.query()
+            assert not waited, "the reset was not on the caller's stream"
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
