@@ -459,7 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     Ring<kKStages> rk;
     Ring<kVStages> rv;
     bool ok = true;
-    float nk = 0.f, nv = 0.f;  // thread 0: scales of the next K block
+    float nk = 0.f, nv = 0.f;  // scales of the next K block
+    float sv = 0.f;            // scale of the next V block
     auto scales = [&](const Item& I, int j) {
       const long long at = (static_cast<long long>(I.b) * p.kv_heads + I.kvh) * p.n_blocks + I.j0 + j;
       nk = p.k_scale[at];
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (true) {
       const Item I = next_item(false, ok);
       if (!ok || I.w < 0) break;
-      if (t == 0 && I.n > 0) scales(I, 0);
+      if (I.n > 0) scales(I, 0);
       for (int jj = 0; ok && jj < 2 * I.n; ++jj, ++g) {
         const bool is_v = (g & 1u) != 0;
         const uint32_t slot = g % kRaw;
@@ -485,8 +486,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(kBarRawEmpty + slot));
-        // What lies past the length may decode to NaN: such keys become zeros.
-        if ((I.j0 + (jj >> 1)) * kBlk + key >= I.len) {
+        // What lies past the length may decode to NaN: such keys become zeros.  So do
+        // the codes of a block whose factor is 0 (a scale of 0, or one whose product
+        // with the softmax scale underflows): its scores, or values, are 0.
+        const float factor = is_v ? sv : nk * p.scale_log2;
+        if ((I.j0 + (jj >> 1)) * kBlk + key >= I.len || !(factor > 0.f)) {
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -508,13 +512,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           st_shared_v4(at + ((u ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
           st_shared_v4(at + (((u + 1) ^ (key & 7)) << 4), h[4], h[5], h[6], h[7]);
         }
-        if (!is_v && t == 0) {
-          // A block whose K scale is 0 has only zero codes: any factor gives its
-          // scores, 0; 1 keeps a masked -inf from meeting 0.
-          st_shared_v4(base + L::kBar + kSlotScale + ((g >> 1) % kScales) * 16,
-                       __float_as_uint(nk > 0.f ? nk * p.scale_log2 : 1.f),
-                       __float_as_uint(nv > 0.f ? __log2f(nv) : kNoScale),
-                       __float_as_uint(nv > 0.f ? __fdividef(1.f, nv) : 8589934592.f), 0u);  // 2^33
+        if (!is_v) {
+          // With 1 in place of a factor of 0 a masked -inf does not meet 0.
+          if (t == 0)
+            st_shared_v4(base + L::kBar + kSlotScale + ((g >> 1) % kScales) * 16,
+                         __float_as_uint(factor > 0.f ? factor : 1.f),
+                         __float_as_uint(nv > 0.f ? __log2f(nv) : kNoScale),
+                         __float_as_uint(nv > 0.f ? __fdividef(1.f, nv) : 8589934592.f), 0u);  // 2^33
+          sv = nv;
           if (jj + 2 < 2 * I.n) scales(I, (jj >> 1) + 1);
         }
         fence_proxy_async_smem();

@@ -419,26 +419,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][i], a0, a1, a2, a3, qf[nt][k][0], qf[nt][k][1]);
           }
-        // A block whose K scale is 0 has only zero codes: any factor gives its
-        // scores, 0; 1 keeps a masked -inf from meeting 0.
-        const float mul = sk > 0.f ? sk * p.scale_log2 : 1.f;
+        // A factor of 0 (a scale of 0, or one whose product with the softmax scale
+        // underflows) makes scores of 0, whatever the codes; with 1 in its place a
+        // masked -inf does not meet 0.  A V scale of 0 makes values of 0.
+        const float factor = sk * p.scale_log2;
+        const float mul = factor > 0.f ? factor : 1.f;
         const float lsv = sv > 0.f ? __log2f(sv) : kNoScale;
         const float isv = sv > 0.f ? __fdividef(1.f, sv) : 8589934592.f;  // 2^33
-        if (key0 + kTileKeys > edge) {
+        if (key0 + kTileKeys > edge || !(fminf(factor, sv) > 0.f)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
+              for (int e = 0; e < 4; ++e) {
+                if (!(factor > 0.f)) s[nt][i][e] *= 0.f;
                 if (key0 + 16 * i + 8 * (e >> 1) + g >= lim[nt][e & 1]) s[nt][i][e] = -INFINITY;
-          if constexpr (FMT == kKv8E4m3) {
-            // What lies past the length may decode to NaN, and 0 * NaN is NaN.
+              }
+          if (FMT == kKv8E4m3 || !(sv > 0.f)) {
+            // What lies past the length may decode to NaN (e4m3), and 0 * NaN is NaN.
+            const int live = sv > 0.f ? len : 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                if (key0 + 16 * i + 2 * c + (x & 1) + (x >> 1) * 8 >= len) {
+                if (key0 + 16 * i + 2 * c + (x & 1) + (x >> 1) * 8 >= live) {
 #pragma unroll
                   for (int k = 0; k < HD / 32; ++k) vw[i][x][k] = 0u;
                 }

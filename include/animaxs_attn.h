@@ -324,8 +324,9 @@ int animaxs_cross_kv_cache_reset(animaxs_cross_kv_cache* cache);
  * A cache is a view of four device buffers that the caller owns:
  *   k_codes, v_codes  [batch][kv_heads][capacity][head_dim], one byte a value
  *   k_scale, v_scale  fp32 [batch][kv_heads][ceil(capacity / 64)]
- * A value is code * scale of its head and 64-token block.  INT8 codes are
- * -127..127, E4M3 codes are 8-bit floats of magnitude <= 448.  The caller keeps
+ * A value is code * scale of its head and 64-token block; a scale is finite and
+ * not negative.  INT8 codes are -127..127, E4M3 codes are 8-bit floats of
+ * magnitude <= 448.  The caller keeps
  * each sequence's length; what lies at or past it does not enter a result, so
  * neither codes nor scales have to be initialised.  A length that counts
  * positions not written yet (a padded batch of prompts, whose later keys a
