@@ -205,6 +205,10 @@ class QuantizedKVCache:
         if q.dtype != torch.float16 or out.dtype != torch.float16 or not (q.is_cuda and out.is_cuda):
             raise _invalid("q and out must be fp16 on the device")
         d.kv_valid_lens = self._ints(lens, "lens")
+        if q_norm_weight is not None and (
+                q_norm_weight.dtype != torch.float16 or q_norm_weight.numel() != self.head_dim
+                or not q_norm_weight.is_cuda or not q_norm_weight.is_contiguous()):
+            raise _invalid(f"q_norm_weight must be a contiguous fp16 device tensor of {self.head_dim} values")
         d.q_norm_weight = None if q_norm_weight is None else q_norm_weight.data_ptr()
         rc = self._lib.animaxs_kv8_attn_forward(self.ex._ctx, self._cref, ctypes.byref(d), q.data_ptr(),
                                                 out.data_ptr(), self._stream(stream))
