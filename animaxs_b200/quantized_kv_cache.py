@@ -107,15 +107,17 @@ class QuantizedKVCache:
         if t is None:
             return None
         import torch
-        if t.dtype != torch.int32 or t.numel() != self.batch or not t.is_cuda or not t.is_contiguous():
-            raise _invalid(f"{what} must be a contiguous int32 device tensor of {self.batch} values")
+        if t.dtype != torch.int32 or t.numel() != self.batch or t.get_device() != self.ex.device \
+                or not t.is_contiguous():
+            raise _invalid(f"{what} must be a contiguous int32 tensor of {self.batch} values on the executor's device")
         return t.data_ptr()
 
     def _view(self, t, tokens, heads, what):
         import torch
-        if t.dtype != torch.float16 or not t.is_cuda or t.dim() != 4 or t.shape[0] != self.batch \
+        if t.dtype != torch.float16 or t.get_device() != self.ex.device or t.dim() != 4 or t.shape[0] != self.batch \
                 or t.shape[2] != heads or t.shape[3] != self.head_dim or (tokens is not None and t.shape[1] != tokens):
-            raise _invalid(f"{what} must be fp16 [{self.batch}, tokens, {heads}, {self.head_dim}] on the device")
+            raise _invalid(f"{what} must be fp16 [{self.batch}, tokens, {heads}, {self.head_dim}] on the "
+                           "executor's device")
         if t.stride(3) != 1:
             raise _invalid("head_dim must be contiguous")
 
@@ -135,8 +137,9 @@ class QuantizedKVCache:
             d = Kv8WriteDesc(k.shape[1], 0, None, None, k.stride(1), k.stride(2), k.stride(0), v.stride(1),
                              v.stride(2), v.stride(0))
             self._remember(key, d)
-        if k.dtype != torch.float16 or v.dtype != torch.float16 or not (k.is_cuda and v.is_cuda):
-            raise _invalid("k and v must be fp16 on the device")
+        dev = self.ex.device
+        if k.dtype != torch.float16 or v.dtype != torch.float16 or k.get_device() != dev or v.get_device() != dev:
+            raise _invalid("k and v must be fp16 on the executor's device")
         d.start = int(start)
         d.starts = self._ints(starts, "starts")
         d.counts = self._ints(counts, "counts")
@@ -202,13 +205,15 @@ class QuantizedKVCache:
             d.q_batch_stride, d.q_tok_stride, d.q_head_stride, _ = q.stride()
             d.o_batch_stride, d.o_tok_stride, d.o_head_stride, _ = out.stride()
             self._remember(key, d)
-        if q.dtype != torch.float16 or out.dtype != torch.float16 or not (q.is_cuda and out.is_cuda):
-            raise _invalid("q and out must be fp16 on the device")
+        dev = self.ex.device
+        if q.dtype != torch.float16 or out.dtype != torch.float16 or q.get_device() != dev or out.get_device() != dev:
+            raise _invalid("q and out must be fp16 on the executor's device")
         d.kv_valid_lens = self._ints(lens, "lens")
         if q_norm_weight is not None and (
                 q_norm_weight.dtype != torch.float16 or q_norm_weight.numel() != self.head_dim
-                or not q_norm_weight.is_cuda or not q_norm_weight.is_contiguous()):
-            raise _invalid(f"q_norm_weight must be a contiguous fp16 device tensor of {self.head_dim} values")
+                or q_norm_weight.get_device() != dev or not q_norm_weight.is_contiguous()):
+            raise _invalid(f"q_norm_weight must be a contiguous fp16 tensor of {self.head_dim} values on the "
+                           "executor's device")
         d.q_norm_weight = None if q_norm_weight is None else q_norm_weight.data_ptr()
         rc = self._lib.animaxs_kv8_attn_forward(self.ex._ctx, self._cref, ctypes.byref(d), q.data_ptr(),
                                                 out.data_ptr(), self._stream(stream))

@@ -105,3 +105,15 @@ def test_norm_weight(cache, weight):
     q, out = Tensor(2, 10, 4, 64), Tensor(2, 10, 4, 64)
     cache.attention(q, out, qk_norm="rms", q_norm_weight=Tensor(64))
     _refused(cache, lambda: cache.attention(q, out, qk_norm="rms", q_norm_weight=weight))
+
+
+@pytest.mark.parametrize("device", [-1, 1])
+@pytest.mark.parametrize("call", ["write k", "write v", "read k", "read v", "attend q", "attend out"])
+def test_tensors_of_another_device(cache, device, call):
+    """The host's, or another GPU's; also where a tensor of the same shape went through before."""
+    for _ in range(2):
+        _refused(cache, _calls(cache, h=Tensor(2, 10, 4, 64, device=device))[call])
+        _refused(cache, _calls(cache, ints=Tensor(2, dtype=torch.int32, device=device))[call])
+        _calls(cache)[call]()
+    _refused(cache, lambda: cache.attention(Tensor(2, 10, 4, 64), Tensor(2, 10, 4, 64), qk_norm="rms",
+                                            q_norm_weight=Tensor(64, device=device)))
