@@ -31,6 +31,14 @@ def _invalid(message):
     return AttentionValidationError(_lib.ERR_INVALID_ARG, message)
 
 
+def _int32(value, what):
+    """``value`` as the C ABI's 32-bit integer; ctypes would drop the bits above without a word."""
+    value = int(value)
+    if not -0x80000000 <= value <= 0x7fffffff:
+        raise AttentionValidationError(_lib.ERR_OVERFLOW, f"{what} {value} does not fit 32 bits")
+    return value
+
+
 class QuantizedKVCache:
     """One layer's K and V of ``batch`` sequences on the executor's device.
 
@@ -46,6 +54,8 @@ class QuantizedKVCache:
         if format not in _FORMATS:
             raise _invalid(f"unknown 8-bit K/V cache format {format!r}")
         code_bytes, scale_bytes = ctypes.c_int64(), ctypes.c_int64()
+        for what, x in (("batch", batch), ("capacity", capacity), ("kv_heads", kv_heads), ("head_dim", head_dim)):
+            _int32(x, what)
         rc = executor._lib.animaxs_kv8_cache_bytes(batch, capacity, kv_heads, head_dim, ctypes.byref(code_bytes),
                                                    ctypes.byref(scale_bytes))
         raise_for(rc, "invalid 8-bit K/V cache shape (head_dim 64 or 128, positive sizes)")
@@ -120,6 +130,7 @@ class QuantizedKVCache:
                            "executor's device")
         if t.stride(3) != 1:
             raise _invalid("head_dim must be contiguous")
+        _int32(t.shape[1], "token count")
 
     def write(self, k, v, start: int = 0, *, starts=None, counts=None, stream=None) -> None:
         """Quantise ``k`` and ``v`` (``[batch, tokens, kv_heads, head_dim]`` fp16, any strides) into positions
@@ -140,7 +151,7 @@ class QuantizedKVCache:
         dev = self.ex.device
         if k.dtype != torch.float16 or v.dtype != torch.float16 or k.get_device() != dev or v.get_device() != dev:
             raise _invalid("k and v must be fp16 on the executor's device")
-        d.start = int(start)
+        d.start = _int32(start, "position")
         d.starts = self._ints(starts, "starts")
         d.counts = self._ints(counts, "counts")
         rc = self._lib.animaxs_kv8_write(self.ex._ctx, self._cref, ctypes.byref(d), k.data_ptr(), v.data_ptr(),
@@ -152,8 +163,11 @@ class QuantizedKVCache:
         """Positions ``[start, start + tokens)`` as fp16 ``(k, v)``, each ``[batch, tokens, kv_heads, head_dim]``;
         rows at or past position ``lens[b]`` are zeros."""
         import torch
-        if tokens is None:
-            tokens = self.capacity - start
+        start = _int32(start, "position")
+        tokens = self.capacity - start if tokens is None else _int32(tokens, "token count")
+        if tokens < 0 or (tokens > 0 and (start < 0 or start + tokens > self.capacity)):
+            raise AttentionValidationError(
+                _lib.ERR_OOB, f"positions [{start}, {start + tokens}) outside the cache's capacity {self.capacity}")
         if k_out is None or v_out is None:
             like = self._descs.get(("r", tokens))  # of the outputs' shape, without memory of its own
             if like is None:
@@ -198,7 +212,7 @@ class QuantizedKVCache:
             if q.shape[1] == 0:
                 return out
             d = self.ex.make_desc(heads=q.shape[2], query_count=q.shape[1],
-                                  key_count=self.capacity if kv_len is None else int(kv_len),
+                                  key_count=self.capacity if kv_len is None else _int32(kv_len, "kv_len"),
                                   head_dim=self.head_dim, key_value_heads=self.kv_heads, causal=causal,
                                   layout=AttentionInputLayout.head_major, qk_norm=qk_norm, qk_norm_targets="q",
                                   eps=eps, scale=scale, batch=self.batch)

@@ -117,3 +117,30 @@ def test_tensors_of_another_device(cache, device, call):
         _calls(cache)[call]()
     _refused(cache, lambda: cache.attention(Tensor(2, 10, 4, 64), Tensor(2, 10, 4, 64), qk_norm="rms",
                                             q_norm_weight=Tensor(64, device=device)))
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 5, -(1 << 32) + 5, 1 << 64])
+def test_integers_past_32_bits(cache, n):
+    """Not cut to their low bits, which name other positions."""
+    h, out = Tensor(2, 10, 4, 64), Tensor(2, 10, 4, 64)
+    for call in (lambda: cache.write(h, h, n), lambda: cache.read(n, 10, k_out=h, v_out=out),
+                 lambda: cache.read(5, n, k_out=h, v_out=out), lambda: cache.read(n, k_out=h, v_out=out),
+                 lambda: cache.attention(h, out, kv_len=n)):
+        _refused(cache, call)
+    if n > 0:
+        wide = Tensor(2, n, 4, 64, stride=(0, 8, 64, 1)) if n < 1 << 60 else h
+        if wide is not h:
+            _refused(cache, lambda: cache.write(wide, wide))
+            _refused(cache, lambda: cache.attention(wide, wide))
+    lib = cache.lib
+    for what in ("batch", "capacity", "kv_heads", "head_dim"):
+        before = len(lib.calls)
+        with pytest.raises(AttentionValidationError):
+            QuantizedKVCache(cache.ex, **{what: n})
+        assert len(lib.calls) == before
+
+
+@pytest.mark.parametrize("start,tokens", [(95, 10), (101, None), (-1, 5), (-5, None), (0, -1), (3, 98)])
+def test_read_outside_the_capacity(cache, start, tokens):
+    """Refused as every other bad argument is, before outputs are made."""
+    _refused(cache, lambda: cache.read(start, tokens))
