@@ -18,13 +18,19 @@ from .executor import AttentionExecutor, AttentionInputLayout
 _FORMATS = {"int8": _lib.KV8_INT8, "e4m3": _lib.KV8_E4M3}
 
 
-try:  # the current stream's handle without a Stream object: 0.1 us of a call that takes 8 in all, not 1.3
-    from torch._C import _cuda_getCurrentRawStream as _current_stream
-except ImportError:
-    import torch
+def _current_stream(device):
+    """The current stream's handle.  The first call finds out how to get it without a Stream object (0.1 us of a call
+    that takes 8 in all, not 1.3), so that importing the package does not import torch."""
+    global _current_stream
+    try:
+        from torch._C import _cuda_getCurrentRawStream as get
+    except ImportError:
+        import torch
 
-    def _current_stream(device):
-        return torch.cuda.current_stream(device).cuda_stream
+        def get(device):
+            return torch.cuda.current_stream(device).cuda_stream
+    _current_stream = get
+    return get(device)
 
 
 def _invalid(message):
