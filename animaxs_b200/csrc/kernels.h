@@ -158,6 +158,11 @@ struct Kv8WriteParams {
   uint8_t* codes[2];
   float* scale[2];
 };
+// 64-token blocks of a head that `tokens` tokens from any start can touch.
+inline long long kv8_write_window(long long tokens, long long capacity) {
+  const long long window = (tokens + kKv8Block - 2) / kKv8Block + 1, all = (capacity + kKv8Block - 1) / kKv8Block;
+  return window < all ? window : all;
+}
 cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream);
 
 struct Kv8ReadParams {

@@ -75,6 +75,9 @@ int check_write(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c, const animaxs
   if ((d->tokens > 1 && (d->k_tok_stride == 0 || d->v_tok_stride == 0)) ||
       (c->kv_heads > 1 && (d->k_head_stride == 0 || d->v_head_stride == 0)))
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "token and head strides must not be 0");
+  // A CTA for K and one for V of every (sequence, head, block).
+  if (2LL * c->batch * c->kv_heads > 0x7fffffffLL / ax::kv8_write_window(d->tokens, c->capacity))
+    return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "8-bit K/V cache write of too many blocks for one call");
   return ANIMAXS_OK;
 }
 
@@ -222,6 +225,8 @@ extern "C" int animaxs_kv8_read(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* 
   if ((tokens > 1 && tok_stride == 0) || (cache->kv_heads > 1 && head_stride == 0) ||
       (cache->batch > 1 && batch_stride == 0))
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "output strides must not be 0");
+  if (2LL * cache->batch * cache->kv_heads > 0x7fffffffLL / ((tokens + ax::kKv8Block - 1LL) / ax::kKv8Block))
+    return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "8-bit K/V cache read of too many blocks for one call");
   DeviceScope scope(ctx->device);
   ax::Kv8ReadParams p{};
   p.format = cache->format;

@@ -236,8 +236,7 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadPar
 }  // namespace
 
 cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream) {
-  // Blocks that `tokens` tokens from any start can touch.
-  const int window = (p.tokens + kKv8Block - 2) / kKv8Block + 1;
+  const int window = static_cast<int>(kv8_write_window(p.tokens, p.capacity));
   const long long ctas = 2LL * window * p.batch * p.kv_heads;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
   auto kernel = p.format == kKv8Int8
@@ -247,7 +246,7 @@ cudaError_t launch_kv8_write(const Kv8WriteParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_kv8_read(const Kv8ReadParams& p, cudaStream_t stream) {
-  const int chunks = (p.tokens + kKv8Block - 1) / kKv8Block;
+  const int chunks = static_cast<int>((p.tokens + kKv8Block - 1LL) / kKv8Block);
   const long long ctas = 2LL * chunks * p.batch * p.kv_heads;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
   auto kernel = p.format == kKv8Int8

@@ -1,0 +1,28 @@
+"""CPU: sizes at which the 8-bit K/V cache's launches reach 32 bits are refused, not cut."""
+import ctypes
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from animaxs_b200 import _lib
+    return _lib.lib()
+
+
+def _write(lib, batch, capacity, kv_heads, tokens):
+    from animaxs_b200._lib import Kv8Cache, Kv8WriteDesc
+    c = Kv8Cache(batch, capacity, kv_heads, 64, 0, 0x1000, 0x2000, 0x3000, 0x4000)
+    d = Kv8WriteDesc(tokens, 0, 0x7000, None, 64 * kv_heads, 64, 1 << 20, 64 * kv_heads, 64, 1 << 20)
+    return lib.animaxs_kv8_write_validate(None, ctypes.byref(c), ctypes.byref(d), 0x5000, 0x6000)
+
+
+@pytest.mark.parametrize("batch,capacity,kv_heads,tokens,code", [
+    (2, 512, 8, (1 << 31) - 1, 0),           # positions past the capacity are not written: 8 blocks a head
+    (2, 512, 8, (1 << 31) - 62, 0),
+    (64, 1 << 30, 8, (1 << 31) - 1, -8),     # 2 x 512 heads x 2^24 blocks
+    (64, 1 << 30, 1, (1 << 31) - 1, -8),
+    (63, 1 << 30, 1, (1 << 31) - 1, 0),
+    (64, 1 << 30, 8, 1 << 20, 0), (1 << 30, 1, 1, 1, -8), ((1 << 30) - 1, 1, 1, 1, 0)])
+def test_blocks_of_a_write(lib, batch, capacity, kv_heads, tokens, code):
+    assert _write(lib, batch, capacity, kv_heads, tokens) == code

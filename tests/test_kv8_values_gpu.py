@@ -78,3 +78,22 @@ def test_a_softmax_scale_that_underflows(ex, fmt, shape, scale):
     out = cache.attention(torch.from_numpy(q).cuda(), lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
                           causal=True, scale=scale)
     _check(out, ora.attention(q, k, v, lens, True, scale), v, keys)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_write_of_more_tokens_than_the_capacity(ex, fmt):
+    """5000 tokens of which the last 50 and 120 fall inside a cache of 100: codes and scales are the definition's."""
+    import torch
+
+    from animaxs_b200 import QuantizedKVCache
+    x = np.random.default_rng(3).standard_normal((2, 5000, 2, 64)).astype(np.float16)
+    cache = QuantizedKVCache(ex, batch=2, capacity=100, kv_heads=2, head_dim=64, format=fmt)
+    starts = [-4950, -4880]
+    dev = torch.from_numpy(x).cuda()
+    cache.write(dev, dev, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    for b in range(2):
+        for h in range(2):
+            values, scale = ora.write(np.zeros((100, 64)), np.zeros(2, np.float32), x[b, :, h], fmt, starts[b], 5000)
+            for codes, s in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+                assert np.array_equal(codes[b, h].double().cpu().numpy(), values)
+                assert np.array_equal(s[b, h].cpu().numpy(), scale)
