@@ -115,8 +115,8 @@ int check_attn(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c, const animaxs_
   r.k_bytes = r.v_bytes = 0;
   rc = ax_validate(ctx, &r, q, c->k_codes, c->v_codes, o);
   if (rc != ANIMAXS_OK) return rc;
-  // A kv head's query rows are numbered in 32 bits.
-  if (static_cast<int64_t>(d->heads) * d->q_len > 0x7fffffffLL)
+  // A kv head's query rows are numbered in 32 bits, up to the end of their last pair of tiles.
+  if (static_cast<int64_t>(d->heads) * d->q_len > 0x7fffffffLL - 2 * ax::kTileM)
     return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "attention byte size overflow");
   return ANIMAXS_OK;
 }

@@ -26,3 +26,16 @@ def _write(lib, batch, capacity, kv_heads, tokens):
     (64, 1 << 30, 8, 1 << 20, 0), (1 << 30, 1, 1, 1, -8), ((1 << 30) - 1, 1, 1, 1, 0)])
 def test_blocks_of_a_write(lib, batch, capacity, kv_heads, tokens, code):
     assert _write(lib, batch, capacity, kv_heads, tokens) == code
+
+
+@pytest.mark.parametrize("heads,q_len,code", [
+    (1, (1 << 31) - 257, 0), (1, (1 << 31) - 256, -8), (1, (1 << 31) - 1, -8), (16, (1 << 27) - 17, 0),
+    (16, (1 << 27) - 1, -8), (4, 1 << 29, -8)])
+def test_query_rows(lib, heads, q_len, code):
+    """Rows are numbered in 32 bits up to the end of the last pair of 128-row tiles."""
+    from animaxs_b200._lib import AttnDesc, Kv8Cache
+    c = Kv8Cache(1, 512, 1, 64, 0, 0x1000, 0x2000, 0x3000, 0x4000)
+    d = AttnDesc()
+    lib.animaxs_attn_desc_init(ctypes.byref(d), 1, heads, 1, q_len, 512, 64)
+    d.q_tok_stride = d.o_tok_stride = 8          # rows that overlap: a view of less memory
+    assert lib.animaxs_kv8_attn_validate(None, ctypes.byref(c), ctypes.byref(d), 0x5000, 0x6000) == code
