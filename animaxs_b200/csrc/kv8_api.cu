@@ -22,6 +22,9 @@ struct DeviceScope {
   }
 };
 
+// Positions are numbered in 32 bits up to the end of the last block.
+constexpr int kMaxCapacity = 0x7fffffff - ax::kKv8Block;
+
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 int check_cache(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c) {
@@ -33,7 +36,7 @@ int check_cache(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c) {
                         c->head_dim);
   if (c->format != ANIMAXS_KV8_INT8 && c->format != ANIMAXS_KV8_E4M3)
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "unknown 8-bit K/V cache format %d", c->format);
-  if (static_cast<int64_t>(c->batch) * c->kv_heads > 0x7fffffffLL ||
+  if (c->capacity > kMaxCapacity || static_cast<int64_t>(c->batch) * c->kv_heads > 0x7fffffffLL ||
       static_cast<__int128>(c->batch) * c->kv_heads * c->capacity * c->head_dim > (static_cast<__int128>(1) << 46))
     return ax_set_error(ctx, ANIMAXS_ERR_OVERFLOW, "attention byte size overflow");
   if (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr || c->v_scale == nullptr)
@@ -159,7 +162,8 @@ extern "C" int animaxs_kv8_cache_bytes(int batch, int capacity, int kv_heads, in
     return ANIMAXS_ERR_INVALID_ARG;
   if (head_dim != 64 && head_dim != 128) return ANIMAXS_ERR_UNSUPPORTED;
   const __int128 heads = static_cast<__int128>(batch) * kv_heads;
-  if (heads * capacity * head_dim > (static_cast<__int128>(1) << 46)) return ANIMAXS_ERR_OVERFLOW;
+  if (capacity > kMaxCapacity || heads * capacity * head_dim > (static_cast<__int128>(1) << 46))
+    return ANIMAXS_ERR_OVERFLOW;
   *code_bytes = static_cast<int64_t>(heads * capacity * head_dim);
   *scale_bytes = static_cast<int64_t>(heads * ((static_cast<int64_t>(capacity) + ax::kKv8Block - 1) / ax::kKv8Block) * 4);
   return ANIMAXS_OK;

@@ -39,3 +39,11 @@ def test_query_rows(lib, heads, q_len, code):
     lib.animaxs_attn_desc_init(ctypes.byref(d), 1, heads, 1, q_len, 512, 64)
     d.q_tok_stride = d.o_tok_stride = 8          # rows that overlap: a view of less memory
     assert lib.animaxs_kv8_attn_validate(None, ctypes.byref(c), ctypes.byref(d), 0x5000, 0x6000) == code
+
+
+@pytest.mark.parametrize("capacity,code", [((1 << 31) - 65, 0), ((1 << 31) - 64, -8), ((1 << 31) - 1, -8)])
+def test_positions(lib, capacity, code):
+    """Positions are numbered in 32 bits up to the end of the last block."""
+    assert _write(lib, 1, capacity, 1, 16) == code
+    a, b = ctypes.c_int64(), ctypes.c_int64()
+    assert lib.animaxs_kv8_cache_bytes(1, capacity, 1, 64, ctypes.byref(a), ctypes.byref(b)) == code
