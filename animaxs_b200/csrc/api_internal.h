@@ -61,6 +61,10 @@ int ax_cuda_fail(animaxs_attn_ctx* ctx, cudaError_t e, const char* what);
 // hold lives until the context is destroyed.
 int ax_grow_buffer(animaxs_attn_ctx* ctx, AxBuffer* buffer, size_t bytes, cudaStream_t stream, const char* what);
 int ax_ensure_scratch(animaxs_attn_ctx* ctx, size_t bytes, cudaStream_t stream);
+// While kernel timing is on: records the start of a launch on `stream` and gives the event
+// that ax_timing_end records behind it (nullptr while it is off).
+int ax_timing_begin(animaxs_attn_ctx* ctx, cudaStream_t stream, cudaEvent_t* stop);
+void ax_timing_end(animaxs_attn_ctx* ctx, cudaStream_t stream, cudaEvent_t stop);
 int ax_validate(animaxs_attn_ctx* ctx, const animaxs_attn_desc* d, const void* q, const void* k,
                 const void* v, const void* o);
 int ax_make_tmap(animaxs_attn_ctx* ctx, CUtensorMap* map, const void* base, int64_t dim, int64_t rows,

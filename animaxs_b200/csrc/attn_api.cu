@@ -372,6 +372,25 @@ extern "C" int animaxs_attn_scratch_bytes(const animaxs_attn_desc* d, int64_t* b
   return ANIMAXS_OK;
 }
 
+int ax_timing_begin(animaxs_attn_ctx* ctx, cudaStream_t stream, cudaEvent_t* stop) {
+  *stop = nullptr;
+  if (!ctx->timing) return ANIMAXS_OK;
+  while (ctx->events.size() < ctx->events_used + 2) {
+    cudaEvent_t ev;
+    cudaError_t ce = cudaEventCreate(&ev);
+    if (ce != cudaSuccess) return ax_cuda_fail(ctx, ce, "timing event");
+    ctx->events.push_back(ev);
+  }
+  cudaEventRecord(ctx->events[ctx->events_used], stream);
+  *stop = ctx->events[ctx->events_used + 1];
+  return ANIMAXS_OK;
+}
+void ax_timing_end(animaxs_attn_ctx* ctx, cudaStream_t stream, cudaEvent_t stop) {
+  if (stop == nullptr) return;
+  cudaEventRecord(stop, stream);
+  ctx->events_used += 2;
+}
+
 // Core of the forward path; `heads_begin/heads_count` select the query heads
 // computed (the head-sharded path uses a sub-range), `o_override` lets the
 // caller redirect the output.
@@ -518,24 +537,12 @@ int ax_forward_range(animaxs_attn_ctx* ctx, const animaxs_attn_desc* d, const vo
     p.peer_go = peers->go;
     p.peer_go_value = peers->go_value;
   }
-  cudaEvent_t ev_start = nullptr, ev_stop = nullptr;
-  if (ctx->timing) {
-    while (ctx->events.size() < ctx->events_used + 2) {
-      cudaEvent_t ev;
-      cudaError_t ce = cudaEventCreate(&ev);
-      if (ce != cudaSuccess) return ax_cuda_fail(ctx, ce, "timing event");
-      ctx->events.push_back(ev);
-    }
-    ev_start = ctx->events[ctx->events_used];
-    ev_stop = ctx->events[ctx->events_used + 1];
-    cudaEventRecord(ev_start, stream);
-  }
+  cudaEvent_t ev_stop = nullptr;
+  rc = ax_timing_begin(ctx, stream, &ev_stop);
+  if (rc != ANIMAXS_OK) return rc;
   cudaError_t e = ax::launch_attn_fwd(tq, tk, tv, p, heads_count, d->batch, stream);
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "attention launch");
-  if (ctx->timing) {
-    cudaEventRecord(ev_stop, stream);
-    ctx->events_used += 2;
-  }
+  ax_timing_end(ctx, stream, ev_stop);
   ctx->query_tiles += static_cast<int64_t>(heads_count) * d->batch *
                       ((d->q_len + ax::kTileM - 1) / ax::kTileM);
   return ANIMAXS_OK;

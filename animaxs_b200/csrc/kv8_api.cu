@@ -341,12 +341,15 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
   if (rc == ANIMAXS_OK) rc = ax_make_tmap_codes(ctx, &tv, cache->v_codes, D, cache->capacity, heads, box);
   if (rc != ANIMAXS_OK) return rc;
   cudaError_t e;
+  cudaEvent_t ev_stop = nullptr;
   if (few) {
     const int grid = ax::kv8_rows_plan(&p, ctx->num_sms);
     rc = ensure_rows_workspace(ctx);
     if (rc != ANIMAXS_OK) return rc;
     p.part = ctx->kv8_rows_part;
     p.count = ctx->kv8_count;
+    rc = ax_timing_begin(ctx, s, &ev_stop);
+    if (rc != ANIMAXS_OK) return rc;
     e = ax::launch_kv8_rows(tk, tv, p, grid, ctx->device, s);
   } else {
     if (!ax::kv8_attn_plan(&p, ctx->num_sms))
@@ -358,10 +361,13 @@ extern "C" int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8
                            ax::kTileM);
     if (rc == ANIMAXS_OK)
       rc = ax_make_tmap_rows(ctx, &to, p.o, D, p.pack, p.q_len, p.lines, p.batch, p.o_tok, p.o_head, p.o_batch, 32);
+    if (rc == ANIMAXS_OK) rc = ax_timing_begin(ctx, s, &ev_stop);
     if (rc != ANIMAXS_OK) return rc;
     e = ax::launch_kv8_attn(tq, tk, tv, to, p, ctx->device, s);
   }
   if (e != cudaSuccess) return ax_cuda_fail(ctx, e, "attention launch");
+  ax_timing_end(ctx, s, ev_stop);
+  ctx->query_tiles += static_cast<int64_t>(d->heads) * d->batch * ((d->q_len + ax::kTileM - 1LL) / ax::kTileM);
   ctx->last_error.clear();
   return ANIMAXS_OK;
 }

@@ -205,8 +205,9 @@ int animaxs_attn_scratch_bytes(const animaxs_attn_desc* desc, int64_t* bytes);
 int animaxs_attn_query_tiles(const animaxs_attn_ctx* ctx, int64_t* tiles);
 
 /* Opt-in GPU timing of the flash-attention kernel: when enabled, every
- * animaxs_attn_forward on this context brackets the attention kernel (not the
- * q/k prologue) with a pair of CUDA events on the caller's stream.
+ * animaxs_attn_forward and animaxs_kv8_attn_forward on this context brackets the
+ * attention kernel (not the q/k prologue; with the join of split keys) with a
+ * pair of CUDA events on the caller's stream.
  * animaxs_attn_kernel_timing waits for the recorded events, returns the
  * launch count, the summed and the largest per-launch time in milliseconds,
  * and clears the record.  Counterpart of the reference's GPU stage timers
