@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/animaxs_attn.h"
 #include "api_internal.h"
@@ -48,6 +49,14 @@ int check_cache(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c) {
   return ANIMAXS_OK;
 }
 
+// Optional DEVICE int32 arrays, one value per sequence.
+int check_ints(animaxs_attn_ctx* ctx, std::initializer_list<const int32_t*> arrays) {
+  for (const int32_t* a : arrays)
+    if (reinterpret_cast<uintptr_t>(a) % 4 != 0)
+      return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "lengths, starts and counts must be 4-byte aligned");
+  return ANIMAXS_OK;
+}
+
 // Strides of an fp16 [batch][tokens][heads][dim] view.
 int check_strides(animaxs_attn_ctx* ctx, std::initializer_list<int64_t> strides) {
   for (int64_t s : strides) {
@@ -67,6 +76,8 @@ int check_write(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c, const animaxs
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "8-bit K/V cache write needs a descriptor, k and v");
   if (misaligned(k) || misaligned(v))
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "8-bit K/V cache write requires 16-byte-aligned k and v");
+  rc = check_ints(ctx, {d->starts, d->counts});
+  if (rc != ANIMAXS_OK) return rc;
   if (d->tokens <= 0) return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "tokens must be positive");
   if (d->starts == nullptr &&
       (d->start < 0 || static_cast<int64_t>(d->start) + (d->counts == nullptr ? d->tokens : 0) > c->capacity))
@@ -104,6 +115,8 @@ int check_attn(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* c, const animaxs_
                         "attention over an 8-bit K/V cache normalises q only (K is normalised before it is written)");
   if (d->numerics == ANIMAXS_NUMERICS_FP32_SCORES_AND_SOFTMAX)
     return ax_set_error(ctx, ANIMAXS_ERR_UNSUPPORTED, "attention over an 8-bit K/V cache has LEGACY numerics only");
+  rc = check_ints(ctx, {d->kv_valid_lens});
+  if (rc != ANIMAXS_OK) return rc;
   if (ctx != nullptr && ctx->score_probe != nullptr)
     return ax_set_error(ctx, ANIMAXS_ERR_UNSUPPORTED, "the score probe does not read an 8-bit K/V cache");
   if (d->batch > 1 && d->o_batch_stride == 0)
@@ -217,6 +230,8 @@ extern "C" int animaxs_kv8_read(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* 
   AxRange range("animaxs_kv8_read");
   if (ctx == nullptr) return ANIMAXS_ERR_INVALID_ARG;
   int rc = check_cache(ctx, cache);
+  if (rc != ANIMAXS_OK) return rc;
+  rc = check_ints(ctx, {lens});
   if (rc != ANIMAXS_OK) return rc;
   if (k_out == nullptr || v_out == nullptr || misaligned(k_out) || misaligned(v_out))
     return ax_set_error(ctx, ANIMAXS_ERR_INVALID_ARG, "8-bit K/V cache read requires 16-byte-aligned outputs");

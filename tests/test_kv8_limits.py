@@ -47,3 +47,18 @@ def test_positions(lib, capacity, code):
     assert _write(lib, 1, capacity, 1, 16) == code
     a, b = ctypes.c_int64(), ctypes.c_int64()
     assert lib.animaxs_kv8_cache_bytes(1, capacity, 1, 64, ctypes.byref(a), ctypes.byref(b)) == code
+
+
+@pytest.mark.parametrize("offset,code", [(0, 0), (4, 0), (1, -1), (2, -1)])
+def test_device_integers_are_aligned(lib, offset, code):
+    """starts, counts and lengths are read as int32: an address between two of them is refused, not read."""
+    from animaxs_b200._lib import AttnDesc, Kv8Cache, Kv8WriteDesc
+    c = Kv8Cache(1, 512, 1, 64, 0, 0x1000, 0x2000, 0x3000, 0x4000)
+    for name in ("starts", "counts"):
+        w = Kv8WriteDesc(16, 0, None, None, 64, 64, 1024, 64, 64, 1024)
+        setattr(w, name, 0x7000 + offset)
+        assert lib.animaxs_kv8_write_validate(None, ctypes.byref(c), ctypes.byref(w), 0x5000, 0x6000) == code
+    d = AttnDesc()
+    lib.animaxs_attn_desc_init(ctypes.byref(d), 1, 1, 1, 3, 512, 64)
+    d.kv_valid_lens = 0x7000 + offset
+    assert lib.animaxs_kv8_attn_validate(None, ctypes.byref(c), ctypes.byref(d), 0x5000, 0x6000) == code
