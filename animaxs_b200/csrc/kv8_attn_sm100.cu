@@ -112,13 +112,6 @@ constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zer
 #define AX_KV8_CONVERT_REGS 80
 #define AX_KV8_OTHER_REGS 80
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2,
                                             int c3, int c4) {
   asm volatile(
