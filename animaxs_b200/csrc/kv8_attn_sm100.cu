@@ -9,7 +9,8 @@
 //
 // Rows: with a power-of-two group the rows of a kv head are its query tokens x
 // the group's heads (row = token * group + head), so that short chunks fill a
-// tile; otherwise every query head is on its own.
+// tile; otherwise every query head is on its own (24 heads x 512 queries on 4096
+// keys, batch 2: 66.3 to 66.9 us with groups of 1, 2, 3 and 4).
 //
 // A work item is a pair of query tiles (A, B) of one (sequence, head line), dealt
 // round-robin to one persistent CTA per SM; where the pairs alone would leave
@@ -31,10 +32,10 @@
 // than 2^8.
 //
 // Measured (GPU time of a call in a graph): 4096 queries x 16 heads on up to 512
-// keys, batch 8 (int8) 103 us; 512 queries x 16 heads on 8704 keys, batch 2 (e4m3,
-// causal) 76 us = 930 TFLOP/s, 0.55 of the measured bf16 peak.  No unit is full:
-// tensor pipe 35 % of active cycles, exp2 32 %, ALU 33 %, shared memory 25 %, DRAM
-// 24 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  Of 2060
+// keys, batch 8 (int8) 104 us; 512 queries x 16 heads on 8704 keys, batch 2 (e4m3,
+// causal) 76.6 us = 923 TFLOP/s, 0.55 of the measured bf16 peak.  No unit is full:
+// tensor pipe 34 % of active cycles, exp2 35 %, ALU 37 %, shared memory 26 %, DRAM
+// 25 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  Of 2060
 // cycles a block (clocks in the kernel) a softmax warp works 1840 (maximum 430,
 // exponentials and P 1130: two tiles share the exp2 unit, 1024), an MMA warp 1425
 // (QK at N = 64 reads 6 KB of shared memory per 32 cycles of MMA).

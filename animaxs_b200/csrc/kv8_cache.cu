@@ -6,9 +6,9 @@
 // one dependent chain (positions -> rows -> maximum -> codes) when there is not.
 //
 // Measured (GPU time of a call in a graph, bytes moved over it; a copy reaches
-// 6.54 TB/s): write of 1 token x 8 heads x 8 sequences 2.35 us, of 8 x 512 tokens
-// x 16 heads 10.1 us = 4.97 TB/s, of 2 x up to 16385 tokens x 8 heads 20.2 us =
-// 5.95 TB/s; read of 32741 tokens x 8 heads 33.2 us = 6.07 TB/s.  The middle
+// 6.54 TB/s): write of 1 token x 8 heads x 8 sequences 2.4 us, of 8 x 512 tokens
+// x 16 heads 10.1 us = 4.98 TB/s, of 2 x up to 16385 tokens x 8 heads 20.1 us =
+// 5.98 TB/s; read of 32741 tokens x 8 heads 32.8 us = 6.13 TB/s.  The middle
 // sizes are a few waves of short CTAs, whose start and end are not hidden.
 // Threads a CTA: 64 and 256 wrote the second in 12.6 and 10.7 us, 128 and 512 read
 // the last in 33.7 and 38.7.

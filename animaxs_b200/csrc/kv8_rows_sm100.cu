@@ -29,10 +29,10 @@
 // order of arrival.
 //
 // Measured (int8, group 2, head_dim 128; GPU time of a call in a graph): batch
-// 1 x 8 kv heads, one query token on 300 keys 4.9 us (equal shares 8.0, of which
-// 3 are the join through global memory), on 2048 keys 5.2 (8.5); a tile costs a
+// 1 x 8 kv heads, one query token on 300 keys 5.1 us (equal shares 8.0, of which
+// 3 are the join through global memory), on 2048 keys 5.5 (8.5); a tile costs a
 // warp 1.4 us when nothing is in flight before it, hence the bound on a
-// cluster's shares.  One token on 131071 keys (e4m3) 52.0 us = 5.17 TB/s, 0.79 of the
+// cluster's shares.  One token on 131071 keys (e4m3) 52.2 us = 5.15 TB/s, 0.79 of the
 // copy rate; the loop alone 0.91.  HBM bounds the loop; around it are 1 us of
 // start, the SMs' spread (+-13 % with equal shares) and 3 us of join.
 //

@@ -2,9 +2,10 @@
 
 Half the memory of an fp16 cache and half the bytes attention reads: ``[batch][kv_heads][capacity][head_dim]``
 codes, int8 or e4m3, for K and for V, with one fp32 scale for each head and block of 64 tokens.  The reference
-has no counterpart (its caches are fp16, AnimaXS/Runtime/Metal/DiTBlockExecutor.swift:19-43); the callers are the
-same: the cross-attention K/V of a block, written once per generation (:1105-1161), and an encoder's cache
-that grows token by token.  The caller keeps each sequence's length.
+has no counterpart (its caches are fp16, AnimaXS/Runtime/Metal/DiTBlockExecutor.swift:19-43).  It serves the
+same cross-attention K/V of a block, written once per generation (:1105-1161), and sequences that grow token
+by token, which the reference does not have (its text encoder runs each prompt in one causal call).  The caller
+keeps each sequence's length.
 """
 
 from __future__ import annotations
@@ -203,8 +204,8 @@ class QuantizedKVCache:
                   qk_norm: str = "none", q_norm_weight=None, eps: float = 1e-6, stream=None):
         """``softmax(scale * q k^T + mask) v`` over the cache for ``q`` ``[batch, q_len, heads, head_dim]`` fp16, any
         strides.  ``kv_len`` (default: the capacity) is the most tokens any sequence has, ``lens`` (int32 device
-        tensor) each one's own length.  ``causal``: the queries are the last ``q_len`` tokens of their sequence.  A query
-        that sees no key gets zeros.  ``qk_norm="rms"`` normalises q first (K is normalised before it is written)."""
+        tensor) each one's own length.  ``causal``: the queries are the last ``q_len`` tokens of their sequence.  A
+        query that sees no key gets zeros.  ``qk_norm="rms"`` normalises q first (K is normalised before it is written)."""
         import torch
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)  # 1 us less than new_empty

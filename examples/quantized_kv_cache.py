@@ -1,8 +1,8 @@
-"""The 8-bit K/V cache at the framework's two callers: ``python examples/quantized_kv_cache.py`` on a B200.
+"""The 8-bit K/V cache in two uses: ``python examples/quantized_kv_cache.py`` on a B200.
 
 * DiT cross-attention: a block's K (RMS-normalised) and V over the adapter context are written once per generation
   and read by every Euler step, from codes instead of fp16.
-* Qwen-shaped decoding (16 query and 8 key/value heads of 128): prompts of different lengths are written in chunks
+* Decoding with the text encoder's heads (16 query and 8 key/value heads of 128): prompts of different lengths are written in chunks
   and attended causally; then every step appends one token to each sequence and attends to all of its cache, replayed
   from one CUDA graph, since positions and lengths are device tensors.
 

@@ -319,8 +319,8 @@ int animaxs_cross_kv_cache_reset(animaxs_cross_kv_cache* cache);
  * A K/V cache in half the memory of fp16, written as tokens arrive, read back,
  * and attended to directly.  No counterpart exists in the reference, whose
  * caches are fp16 (CrossKVCache, DiTBlockExecutor.swift:19-43); it serves the
- * same callers: the cross-attention K/V of every block, written once per
- * generation, and a text encoder's cache that grows token by token.
+ * same cross-attention K/V of every block, written once per generation, and
+ * sequences that grow token by token, which the reference does not have.
  *
  * A cache is a view of four device buffers that the caller owns:
  *   k_codes, v_codes  [batch][kv_heads][capacity][head_dim], one byte a value
@@ -375,8 +375,8 @@ typedef struct animaxs_kv8_write_desc {
 int animaxs_kv8_write(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
                       const animaxs_kv8_write_desc* desc, const void* k, const void* v, void* stream);
 
-/* Read positions [start, start + tokens) back as fp16, code * scale rounded
- * once, into k_out and v_out ([batch][tokens][kv_heads][head_dim], one set of
+/* Read positions [start, start + tokens) back as fp16 (code * scale in fp32,
+ * then rounded to fp16) into k_out and v_out ([batch][tokens][kv_heads][head_dim], one set of
  * element strides for both).  `lens` (optional DEVICE int32[batch]): rows at
  * or past position lens[b] are stored as zeros. */
 int animaxs_kv8_read(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache, int start, int tokens,
@@ -395,7 +395,16 @@ int animaxs_kv8_read(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache, int 
  * own.  A query that sees no key gets zeros.  Scores, softmax statistics and
  * accumulators are fp32, probabilities enter the second product as fp16.
  * Head dims 64 and 128, numerics LEGACY; with a score probe set the call
- * returns ANIMAXS_ERR_UNSUPPORTED. */
+ * returns ANIMAXS_ERR_UNSUPPORTED.
+ * The context allocates its workspaces at the first call that uses each (up to
+ * 16 query rows of a kv head; more rows with split keys), so make one call of
+ * the same shape before a stream capture.  They fit every shape and stay until the
+ * context is destroyed, and so does the scratch of a captured qk_norm call: later
+ * calls leave a captured graph valid.  Calls that use one context at the same
+ * time (on several streams, or a replay beside a call) would share them.
+ * Equal calls give equal bits.  How the keys are shared out over the SMs follows from
+ * the shapes, kv_len and, with up to 16 rows, the lengths of all sequences,
+ * so a sequence's last bits may change when another one of the batch grows. */
 int animaxs_kv8_attn_forward(animaxs_attn_ctx* ctx, const animaxs_kv8_cache* cache,
                              const animaxs_attn_desc* desc, const void* q, void* o, void* stream);
 
