@@ -105,7 +105,6 @@ constexpr uint32_t kSlotItem = kSlotScale + kScales * 16;  // Item [kItems]
 static_assert(kSlotAbort + 4 <= kSlotScale && kSlotItem + kItems * 48 <= kBarBytes, "barrier block overflows");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 256;
-constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
 // Register split (setmaxnreg) of the 512 x 128 registers of the launch: softmax
 // 2 x 128 threads, conversion 128, MMA / TMA 128 (build.py checks the sum).
@@ -483,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // What lies past the length may decode to NaN: such keys become zeros.  So do
         // the codes of a block whose factor is 0 (a scale of 0, or one whose product
         // with the softmax scale underflows): its scores, or values, are 0.
-        const float factor = is_v ? sv : nk * p.scale_log2;
+        const float factor = is_v ? (sv > kKv8NoValue ? sv : 0.f) : nk * p.scale_log2;
         if ((I.j0 + (jj >> 1)) * kBlk + key >= I.len || !(factor > 0.f)) {
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -511,8 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t == 0)
             st_shared_v4(base + L::kBar + kSlotScale + ((g >> 1) % kScales) * 16,
                          __float_as_uint(factor > 0.f ? factor : 1.f),
-                         __float_as_uint(nv > 0.f ? __log2f(nv) : kNoScale),
-                         __float_as_uint(nv > 0.f ? __fdividef(1.f, nv) : 8589934592.f), 0u);  // 2^33
+                         __float_as_uint(nv > kKv8NoValue ? __log2f(nv) : kKv8NoScale),
+                         __float_as_uint(nv > kKv8NoValue ? __fdividef(1.f, nv) : kKv8NoScaleInverse), 0u);
           sv = nv;
           if (jj + 2 < 2 * I.n) scales(I, (jj >> 1) + 1);
         }

@@ -20,6 +20,14 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
 }
 
+// A V scale up to this stands for 0: its values vanish in an fp16 output, while the
+// weights of its keys have to count, and 1 / scale and the probabilities scaled by
+// it would leave the range of fp32.
+constexpr float kKv8NoValue = 8.27180613e-25f;  // 2^-80
+// Stands for log2 of such a scale (below that of any written block, 2^-33).
+constexpr float kKv8NoScale = -33.f;
+constexpr float kKv8NoScaleInverse = 8589934592.f;  // 2^33
+
 // Four codes (one per byte of w) -> half2 of bytes 0, 1 and half2 of bytes 2, 3.
 // int8: code + 128 is placed under the exponent of 1024 (0x64xx = 1024 + xx)
 // and 1152 is subtracted, all exact: 1.25 instructions a value.

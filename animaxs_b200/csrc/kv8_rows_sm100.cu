@@ -59,7 +59,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTileKeys = 32;
 constexpr int kAlone = 3;          // tiles of a warp up to which a line has a cluster of its own (kv8_rows_plan)
 constexpr float kRescale = 8.f;    // log2 units by which the maximum may lag
-constexpr float kNoScale = -33.f;  // stands for log2 of the scale of an all-zero V block (below any real one)
 
 // What a slot holds: the line's first tile (-1: nothing), sequence, kv head and tiles.
 struct alignas(16) SlotInfo {
@@ -417,9 +416,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         // masked -inf does not meet 0.  A V scale of 0 makes values of 0.
         const float factor = sk * p.scale_log2;
         const float mul = factor > 0.f ? factor : 1.f;
-        const float lsv = sv > 0.f ? __log2f(sv) : kNoScale;
-        const float isv = sv > 0.f ? __fdividef(1.f, sv) : 8589934592.f;  // 2^33
-        if (key0 + kTileKeys > edge || !(fminf(factor, sv) > 0.f)) {
+        const bool valued = sv > kKv8NoValue;
+        const float lsv = valued ? __log2f(sv) : kKv8NoScale;
+        const float isv = valued ? __fdividef(1.f, sv) : kKv8NoScaleInverse;
+        if (key0 + kTileKeys > edge || !(factor > 0.f) || !valued) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -429,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(factor > 0.f)) s[nt][i][e] *= 0.f;
                 if (key0 + 16 * i + 8 * (e >> 1) + g >= lim[nt][e & 1]) s[nt][i][e] = -INFINITY;
               }
-          if (FMT == kKv8E4m3 || !(sv > 0.f)) {
+          if (FMT == kKv8E4m3 || !valued) {
             // What lies past the length may decode to NaN (e4m3), and 0 * NaN is NaN.
-            const int live = sv > 0.f ? len : 0;
+            const int live = valued ? len : 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -97,3 +97,24 @@ def test_a_write_of_more_tokens_than_the_capacity(ex, fmt):
             for codes, s in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
                 assert np.array_equal(codes[b, h].double().cpu().numpy(), values)
                 assert np.array_equal(s[b, h].cpu().numpy(), scale)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", SHAPES, ids=[str(i) for i in range(len(SHAPES))])
+@pytest.mark.parametrize("tiny", [1e-20, 1e-30, 2e-38, 1e-38, 1e-40, 1e-45])
+def test_a_v_scale_that_makes_values_vanish(ex, fmt, shape, tiny):
+    """Blocks of zeros often come with the least scale that a quantiser divides by (fp32's least normal / 127, say):
+    their values add nothing that fp16 holds, but their keys keep their weights."""
+    import torch
+    batch, q_len, heads, kv_heads, dim, keys = shape
+    cache, k, v = _wrapped(ex, fmt, batch, kv_heads, keys, dim, keys)
+    blocks = cache.v_scale.shape[2]
+    cache.v_scale[:, :, 0::2] = tiny
+    if blocks > 1:
+        cache.v_scale[:, :, 1::2] = 0.01
+    v = ora.decode(cache.v_codes.double().cpu().numpy(), cache.v_scale.cpu().numpy())
+    q = np.random.default_rng(keys + 1).standard_normal((batch, q_len, heads, dim)).astype(np.float16)
+    lens = [keys - 45 * i for i in range(batch)]
+    out = cache.attention(torch.from_numpy(q).cuda(), lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                          causal=True)
+    _check(out, ora.attention(q, k, v, lens, True), v, keys)
