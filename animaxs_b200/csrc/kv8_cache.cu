@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
 #pragma unroll
   for (int i = 0; i < kWriteThreads / 32; ++i) a = fmaxf(a, warp_max[i]);
   const float s = fmaxf(__fmul_rn(a, 1.f / kKv8Top<FMT>), before);
-  const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+  // A scale that a caller put there may be so small that 1 / s overflows; only values of
+  // 0 meet it, whose codes are 0.
+  const float inv = s > 0.f ? fminf(__fdiv_rn(1.f, s), 3.402823466e38f) : 0.f;
   if (finite) {
     // With a scale of 0 every finite value is 0, and 0 * 0 rounds to code 0.
 #pragma unroll

@@ -118,3 +118,28 @@ def test_a_v_scale_that_makes_values_vanish(ex, fmt, shape, tiny):
     out = cache.attention(torch.from_numpy(q).cuda(), lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
                           causal=True)
     _check(out, ora.attention(q, k, v, lens, True), v, keys)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("scale", [1e-38, 1e-39, 1e-45])
+def test_zeros_behind_a_vanishing_scale(ex, fmt, scale):
+    """Tokens of zeros appended to a block whose scale is so small that its inverse overflows: codes of 0, the older
+    ones and the scale as they were; values that are not zero take the scale over."""
+    import torch
+
+    from animaxs_b200 import QuantizedKVCache
+    cache = QuantizedKVCache(ex, batch=1, capacity=128, kv_heads=2, head_dim=64, format=fmt)
+    for codes, s in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+        codes[:, :, :10].copy_(torch.full((1, 2, 10, 64), 3.0, device="cuda").to(codes.dtype))
+        codes[:, :, 10:].view(torch.uint8).fill_(0x55)
+        s.fill_(scale)
+    held = cache.k_scale.clone()
+    zeros = torch.zeros((1, 20, 2, 64), dtype=torch.float16, device="cuda")
+    cache.write(zeros, zeros, 10)
+    for codes, s in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+        assert (codes[:, :, 10:30].float() == 0).all() and (codes[:, :, :10].float() == 3).all()
+        assert torch.equal(s, held)
+    ones = torch.ones((1, 1, 2, 64), dtype=torch.float16, device="cuda")
+    cache.write(ones, ones, 30)
+    top = 127 if fmt == "int8" else 448
+    assert (cache.k_codes[:, :, 30].float() == top).all() and (cache.k_codes[:, :, :30].float() == 0).all()
