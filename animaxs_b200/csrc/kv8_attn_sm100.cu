@@ -35,7 +35,7 @@
 // keys, batch 8 (int8) 104 us; 512 queries x 16 heads on 8704 keys, batch 2 (e4m3,
 // causal) 76.6 us = 923 TFLOP/s, 0.55 of the measured bf16 peak.  No unit is full:
 // tensor pipe 34 % of active cycles, exp2 35 %, ALU 37 %, shared memory 26 %, DRAM
-// 25 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  Of 2060
+// 24 %; half the QK MMAs gained 4 %, no exp2 5 %, no conversion stores 1 %.  Of 2060
 // cycles a block (clocks in the kernel) a softmax warp works 1840 (maximum 430,
 // exponentials and P 1130: two tiles share the exp2 unit, 1024), an MMA warp 1425
 // (QK at N = 64 reads 6 KB of shared memory per 32 cycles of MMA).
